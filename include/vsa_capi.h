@@ -451,6 +451,96 @@ int vsa_op_fwd(const vsa_op* op, void* out, void* saved, void* scratch, void* st
 int vsa_op_bwd(const vsa_op* op, const void* out, const void* dout, void* saved, void* scratch,
                void* dq, void* dk, void* dv, void* d_gate, void* stream);
 
+/*
+ * Rotary positions (no counterpart in the reference, whose operators take q and
+ * k as they are: these turn them before the attention).
+ *
+ * A latent grid's table: token (t, h, w) of a row-major T x H x W grid gets, for
+ * every pair of channels of every axis, cos and sin of (start + index) * f,
+ * f_i = theta^(-2 i / channels) scaled by `method`:
+ *  - VSA_ROTARY_LINEAR: f / factor (positions interpolated);
+ *  - VSA_ROTARY_NTK: theta * factor^(channels / (channels - 2)) in theta's place;
+ *  - VSA_ROTARY_YARN (Peng et al. 2023): f * g + f / factor * (1 - g) with g the
+ *    ramp (original * f / 2 pi - 1) / 31 clamped to [0, 1], and cos and sin
+ *    times 0.1 ln(factor) + 1.
+ * The axes' pairs follow each other; an axis may have 0 channels, all together
+ * at most 256.  Angles are made in 64 bits.  axes is host memory (three
+ * entries, read before the call returns); cos_out and sin_out are
+ * [T*H*W, sum(channels) / 2].
+ */
+enum vsa_rotary_method { VSA_ROTARY_LINEAR = 0, VSA_ROTARY_NTK = 1, VSA_ROTARY_YARN = 2 };
+
+typedef struct vsa_rotary_axis {
+  int32_t positions, channels, method, reserved;
+  double start, theta, factor, original;   /* original: yarn alone */
+} vsa_rotary_axis;
+
+int vsa_rotary_table(const vsa_rotary_axis* axes, float* cos_out, float* sin_out, void* stream);
+
+/*
+ * q_out, k_out = q, k with the first `channels` of each head turned by the rows
+ * of a table ([rows, channels / 2]): pairs (i, i + channels / 2), or (2i, 2i + 1)
+ * with `interleaved`; by the opposite angle with `inverse` (the gradient).  The
+ * other channels are copied.  Token t of every sample takes row t, or row
+ * positions[b * positions_stride + t] (int32, int64 with positions64): the token
+ * is copied as it is for a negative one and becomes NaN for one past the table.
+ * Strides are those of batch, head and token in elements; channels lie next to
+ * each other.  k and k_out are ignored with k_heads 0.  Any alignment of the
+ * element type; rows that start 16-byte aligned run fastest.
+ */
+typedef struct vsa_rotary_op {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const float *cos_table, *sin_table;
+  const void* positions;
+  int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];
+  int64_t positions_stride, batch, tokens, rows;
+  int32_t q_heads, k_heads, head_dim, channels, interleaved, inverse, positions64, dtype;
+} vsa_rotary_op;
+
+int vsa_rotary(const vsa_rotary_op* op, void* stream);
+
+/*
+ * Cross attention to an encoder's states (no counterpart in the reference):
+ * out = softmax(scale q k^T over the sample's valid keys) v.  q is [batch, heads,
+ * sq, head_dim], k and v [batch, kv_heads, skv, head_dim], heads a multiple of
+ * kv_heads, by strides of batch, head and token in elements (0 for a broadcast
+ * one); channels lie next to each other, rows start 16-byte aligned, head_dim is
+ * a multiple of 8 up to 256.  A key is valid if it lies below kv_lens[b] (NULL:
+ * all; clamped to [0, skv]) and key_mask[b * mask_stride + key] is not zero
+ * (NULL: all).  What lies behind a key that is not valid has no influence, NaN
+ * included.  A sample without a valid key gets zeros, and zero gradients.
+ *
+ * lse (fp32 [batch, heads, sq], NULL: not wanted) is the base-2 log-sum-exp the
+ * backward needs, -inf without a valid key; lo ([batch, heads, sq, head_dim],
+ * dense, 16-byte aligned; NULL: not wanted) is what rounding out to bf16 / fp16
+ * left over, which a backward with it takes its row sums of dout * out from
+ * (without it dq loses up to two bits; unused in fp32).  dk and dv are written for every
+ * key (zeros where it is not valid) and summed over the heads that share a key
+ * head, in a fixed order.  Scratch sizes come from vsa_cross_sizes (256-byte
+ * aligned; 0: NULL will do).
+ */
+typedef struct vsa_cross {
+  const void *q, *k, *v;
+  const int32_t* kv_lens;
+  const void* key_mask;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int64_t mask_stride, sq, skv;
+  int32_t batch, heads, kv_heads, head_dim, dtype;
+  float scale;
+} vsa_cross;
+
+int vsa_cross_sizes(const vsa_cross* c, int64_t* scratch_fwd, int64_t* scratch_bwd);
+
+int vsa_cross_fwd(const vsa_cross* c, void* out, const int64_t* out_stride, void* lo, float* lse,
+                  void* scratch, void* stream);
+
+int vsa_cross_bwd(const vsa_cross* c, const void* out, const int64_t* out_stride,
+                  const void* lo, const void* dout, const int64_t* dout_stride, const float* lse,
+                  void* dq,
+                  const int64_t* dq_stride, void* dk, const int64_t* dk_stride, void* dv,
+                  const int64_t* dv_stride, void* scratch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,305 @@
+// Cross attention on gfx950: what the forward and the backward share.
+//
+//   O = softmax(scale Q K^T over the sample's valid keys) V
+//
+// q rows are [batch, heads, sq], k / v rows [batch, kv_heads, skv], any strides
+// with the channels next to each other and 16-byte aligned rows.  The heads of
+// a group (heads / kv_heads) share a key head.  A key is valid if it lies below
+// its sample's kv_lens and its key_mask byte is not zero.
+//
+// Tiles of K and V (or Q and dO) are copied to LDS by direct loads; the rows of
+// keys that are not valid, and the channels past the head dim, are fetched from
+// 16 bytes of zeros instead, so that nothing behind a mask (infinities, NaN,
+// memory past the last row) takes part in a product.
+#pragma once
+
+#include "vsa_device.h"
+#include "vsa_launch.h"
+
+namespace vsa {
+
+// 32x32 products over 16 elements of the reduced axis, per element type.  fp32
+// takes v_mfma_f32_32x32x2_f32: element e of the two operands is the pair of
+// reduced elements e and 8 + e of lane halves 0 and 1, the same pairing on both
+// sides, so any order of the 16 does.
+template <typename T>
+struct Mma {
+  typedef typename Elem<T>::vec8 V8;
+  static __device__ __forceinline__ f32x16 mul(V8 a, V8 b, f32x16 c) {
+    return Elem<T>::mfma32(a, b, c);
+  }
+};
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+template <>
+struct Mma<float> {
+  typedef f32x8 V8;
+  static __device__ __forceinline__ f32x16 mul(V8 a, V8 b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::V8 pack_op(const float* v) {
+  if constexpr (sizeof(T) == 4) {
+    f32x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = v[e];
+    return r;
+  } else {
+    return pack8<T>(v);
+  }
+}
+
+// 8 consecutive elements at a 16-byte aligned address
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::V8 ld8(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  } else {
+    return as_vec8<T>(*reinterpret_cast<const u32x4*>(p));
+  }
+}
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::V8 zero8() {
+  typename Mma<T>::V8 z = {};
+  return z;
+}
+
+// fp32 at head dim 256 leaves no registers to read operands ahead: without a
+// fence after each step of a product the compiler moves the reads of all of
+// them to the front and spills.
+template <typename T, int D>
+__device__ __forceinline__ void step_fence() {
+  if constexpr (D * sizeof(T) > 512) __builtin_amdgcn_sched_barrier(0);
+}
+
+// LDS tile of rows of D elements, 16-byte chunks swizzled by the row: 16-bit
+// types as in vsa_device.h, fp32 rows (at least 256 bytes: one pass over the 64
+// banks) by the row's low four bits.
+template <typename T, int D>
+struct Tile {
+  static constexpr int CH = D * (int)sizeof(T) / 16;  // chunks of a row
+  static constexpr int ROW = D * (int)sizeof(T);      // bytes of a row
+  static __device__ __forceinline__ int off(int r, int c) {
+    if constexpr (sizeof(T) == 2) return swz<D>(r, c) * 2;
+    else return r * ROW + ((c >> 4) << 8) + (((c & 15) ^ (r & 15)) << 4);
+  }
+  // row and chunk that live at chunk position P
+  static __device__ __forceinline__ int unoff(int P, int& c) {
+    if constexpr (sizeof(T) == 2) {
+      return unswz_row_chunk<D>(P, c);
+    } else {
+      const int r = P / CH;
+      c = (P % CH) ^ (r & 15);   // the upper bits of a chunk stay
+      return r;
+    }
+  }
+};
+
+// Row operand: lane (r, h) takes elements 16 ks + 8 h .. + 7 of row `row`.
+template <typename T, int D>
+__device__ __forceinline__ typename Mma<T>::V8 row_op(const char* X, int row, int ks, int h) {
+  typedef Tile<T, D> L;
+  if constexpr (sizeof(T) == 2) {
+    return as_vec8<T>(*reinterpret_cast<const u32x4*>(X + L::off(row, 2 * ks + h)));
+  } else {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(X + L::off(row, 4 * ks + 2 * h));
+    const f32x4 b = *reinterpret_cast<const f32x4*>(X + L::off(row, 4 * ks + 2 * h + 1));
+    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+}
+
+// Column operand: lane (r, h) takes channel d0 + r of rows s + 4h .. + 3 and
+// s + 8 + 4h .. + 3, the order in which a 32x32 result holds its rows.
+template <typename T, int D>
+__device__ __forceinline__ typename Mma<T>::V8 col_op(const char* X, int d0, int s) {
+  if constexpr (sizeof(T) == 2) {
+    return tr_a8<T, D>(reinterpret_cast<const T*>(X), d0, s, s + 8);
+  } else {
+    typedef Tile<T, D> L;
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    f32x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = s + (e >> 2) * 8 + 4 * h + (e & 3);
+      // chunk d0 / 4 + r / 4: d0 is a multiple of 32, so its bits above the low
+      // three of r / 4 can be split off
+      const int lo = ((d0 >> 2) & 8) | (r >> 2);
+      v[e] = *reinterpret_cast<const float*>(X + row * L::ROW + ((d0 >> 6) << 8) +
+                                             ((lo ^ (row & 15)) << 4) + (r & 3) * 4);
+    }
+    return v;
+  }
+}
+
+// What copies of masked rows and of channels past the head dim read, and what
+// the statistics of query rows past the last one read: P = 2^(s - inf) = 0.
+__device__ __attribute__((aligned(16))) static const uint32_t kZero16[4] = {0, 0, 0, 0};
+__device__ __attribute__((aligned(16))) static const float kPastStats[2] = {INFINITY, 0.f};
+
+// Copies ROWS rows of D elements into a tile, as NT threads.  Rows whose bit of
+// `valid` is clear become zeros, and so do channels past `dim`.  The byte
+// offsets of a thread's pieces are kept in registers where there are up to
+// eight of them; more are worked out again for each copy.
+template <typename T, int D, int ROWS, int NT>
+struct TileCopy {
+  typedef Tile<T, D> L;
+  static constexpr int N = ROWS * L::CH / NT;  // 16-byte pieces of a thread
+  static constexpr bool KEEP = N <= 8;
+  static_assert(ROWS * L::CH % NT == 0 && ROWS % 32 == 0, "");
+  uint32_t voff[KEEP ? N : 1];   // byte offset of the piece from the tile's first row
+  uint32_t stride;               // bytes between rows
+  int dim;                       // bytes of a row
+
+  static __device__ __forceinline__ int place(int i, int tid, int& c) {
+    return L::unoff(i * NT + tid, c);
+  }
+  __device__ __forceinline__ uint32_t offset(int i, int tid) const {
+    int c;
+    const int row = place(i, tid, c);
+    return (uint32_t)row * stride + (uint32_t)c * 16u;
+  }
+  __device__ __forceinline__ void init(int64_t row_stride, int channels) {
+    stride = (uint32_t)(row_stride * (int)sizeof(T));
+    dim = channels * (int)sizeof(T);
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) voff[i] = opaque(offset(i, threadIdx.x));
+    }
+  }
+  static __device__ __forceinline__ uint32_t lds_base(uint32_t lds) {
+    return lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024u;
+  }
+  // every row valid, every channel within the head dim
+  __device__ __forceinline__ void whole(uint32_t lds, const T* src) const {
+    const uint32_t base = lds_base(lds);
+    const int tid = KEEP ? 0 : opaque((int)threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      dma16_s(KEEP ? voff[KEEP ? i : 0] : offset(i, tid), src, base + (uint32_t)i * (NT / 64) * 1024u);
+  }
+  __device__ __forceinline__ void part(uint32_t lds, const T* src,
+                                       const uint32_t (&valid)[ROWS / 32]) const {
+    const uint32_t base = lds_base(lds);
+    const int tid = opaque((int)threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int c;
+      const int row = place(i, tid, c);
+      uint32_t w = valid[0];
+#pragma unroll
+      for (int x = 1; x < ROWS / 32; ++x) w = row >= 32 * x ? valid[x] : w;
+      const bool on = ((w >> (row & 31)) & 1u) != 0 && c * 16 < dim;
+      const char* g = on ? reinterpret_cast<const char*>(src) + offset(i, tid)
+                         : reinterpret_cast<const char*>(kZero16);
+      dma16(g, base + (uint32_t)i * (NT / 64) * 1024u);
+    }
+  }
+};
+
+struct Rows {          // a [batch, head, token] view
+  const void* p;
+  int64_t b, h, s;     // strides in elements
+};
+
+struct CrossArgs {
+  Rows q, k, v, o, dout;
+  void *out, *dq, *dk, *dv;
+  void *lo;                    // what rounding the output left over, [batch, heads, sq, dim], or null
+  int64_t out_s[3], dq_s[3], dk_s[3], dv_s[3];
+  float *lse, *delta;          // [batch, heads, sq]
+  float *part_a, *part_b;      // fp32 partial results of the splits
+  const int32_t* lens;
+  const uint32_t* words;       // [batch, nwords] of 32 keys, or null
+  int nwords;
+  int sq, skv, heads, kv_heads, group, dim;
+  int batch, splits, tiles;    // tiles of a split
+  int per_head;                // tiles of a (batch, key head)
+  float c2, scale;
+  uint32_t qsign;
+};
+
+typedef const __attribute__((address_space(4))) uint32_t* const_words;
+
+// The chunks of KC keys of one sample that hold a valid key, in order.  The
+// words are read through the constant address space: scalar loads, which the
+// direct copies' vmcnt waits never include.
+template <int KC>
+struct KeyWalk {
+  const_words words;
+  int n, last;               // valid prefix; chunk past the last one
+  int j;
+  uint32_t w[KC / 32];
+
+  __device__ __forceinline__ void init(const CrossArgs& a, int b, int first, int chunks) {
+    n = a.skv;
+    if (a.lens) n = min(max(a.lens[b], 0), a.skv);
+    n = __builtin_amdgcn_readfirstlane(n);
+    words = a.words ? (const_words)(uintptr_t)(a.words + (int64_t)b * a.nwords) : nullptr;
+    j = first;
+    last = min(first + chunks, (n + KC - 1) / KC);
+  }
+  // The next chunk with a valid key at or after j; false if there is none.
+  __device__ __forceinline__ bool find() {
+    for (; j < last; ++j) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int x = 0; x < KC / 32; ++x) {
+        const int left = n - j * KC - 32 * x;
+        w[x] = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u;
+        if (words) w[x] &= words[j * (KC / 32) + x];
+        any |= w[x];
+      }
+      if (any) return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool whole() const {
+    uint32_t all = ~0u;
+#pragma unroll
+    for (int x = 0; x < KC / 32; ++x) all &= w[x];
+    return all == ~0u;
+  }
+};
+
+// valid bit of the key that accumulator element i of lane half h holds
+__device__ __forceinline__ bool acc_valid(uint32_t w, int i, int h) {
+  return (w >> (8 * (i >> 2) + 4 * h + (i & 3))) & 1u;
+}
+
+// Eight consecutive channels of a row, as T.
+template <typename T>
+__device__ __forceinline__ void st8(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    T o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = Elem<T>::from_f(v[e]);
+    *reinterpret_cast<u32x4*>(p) = *reinterpret_cast<const u32x4*>(o);
+  }
+}
+
+// Eight channels of the output, and what rounding them to T left over: delta is
+// sum dO O, and where the weights are spread over many keys dS = P (dP - delta)
+// is so much smaller than dP that the rounding of O shows in dQ (bf16, 4000
+// keys: 6.6e-3 of its norm, 1e-5 with the rest; the roundings that stay, of dS
+// and of dQ, make 2.4e-3).
+template <typename T>
+__device__ __forceinline__ void st8_out(T* out, T* lo, const float (&v)[8]) {
+  st8<T>(out, v);
+  if constexpr (sizeof(T) == 2) {
+    if (lo) {
+      float rest[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) rest[e] = v[e] - round_t<T>(v[e]);
+      st8<T>(lo, rest);
+    }
+  }
+}
+
+}  // namespace vsa

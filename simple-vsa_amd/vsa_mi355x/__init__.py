@@ -14,10 +14,13 @@ reference's names (vsa/__init__.py:7, 10-25).
 from typing import Any
 
 from .gate import CompressionGate
+from .rotary import build_rotary_table
 from .tiling import build_vsa_metadata, tile, untile
 
 __all__ = ["mi355x_vsa", "mi355x_sparse_attention", "mi355x_sparse_executor", "mi355x_route",
-           "mi355x_vsa_tiled", "CompressionGate", "build_vsa_metadata", "tile", "untile"]
+           "mi355x_vsa_tiled", "mi355x_rotary", "mi355x_cross_attention", "CompressionGate",
+           "build_vsa_metadata",
+           "build_rotary_table", "tile", "untile"]
 
 
 def mi355x_vsa(*args: Any, **kwargs: Any) -> Any:
@@ -52,5 +55,20 @@ def mi355x_vsa_tiled(*args: Any, **kwargs: Any) -> Any:
     """VSA on raster-order video tokens with tile / untile fused into the op;
     see ``vsa_mi355x.tiled``."""
     from .tiled import mi355x_vsa_tiled as _impl
+
+    return _impl(*args, **kwargs)
+
+
+def mi355x_rotary(*args: Any, **kwargs: Any) -> Any:
+    """q and k turned by the rotary positions of their tokens; see
+    ``vsa_mi355x.rotary``."""
+    from .rotary import mi355x_rotary as _impl
+
+    return _impl(*args, **kwargs)
+
+
+def mi355x_cross_attention(*args: Any, **kwargs: Any) -> Any:
+    """Attention to an encoder's states of another length; see ``vsa_mi355x.cross``."""
+    from .cross import mi355x_cross_attention as _impl
 
     return _impl(*args, **kwargs)

@@ -66,6 +66,12 @@ SIGNATURES = {
     "vsa_sparse_bwd_dkdv_tiled": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                   _I64, _I32, _I64, _I64, _I64, _I32, _I32, _I32, _F, _P, _I32,
                                   _P],
+    # rotary positions and cross attention
+    "vsa_rotary_table": [_P, _P, _P, _P],
+    "vsa_rotary": [_P, _P],
+    "vsa_cross_sizes": [_P, _P, _P],
+    "vsa_cross_fwd": [_P] * 7,
+    "vsa_cross_bwd": [_P] * 15,
 }
 _RESTYPES = {"vsa_status_string": ctypes.c_char_p, "vsa_version": ctypes.c_char_p}
 
@@ -78,6 +84,31 @@ class VsaOp(ctypes.Structure):
                 + [(n, _I32) for n in ("heads", "head_dim", "block", "kernel_dim",
                                        "kernel_block", "topk", "gate_mode", "gate_heads",
                                        "dtype", "keep")]
+                + [("scale", _F)])
+
+
+class VsaRotaryAxis(ctypes.Structure):
+    """``struct vsa_rotary_axis`` of the header."""
+    _fields_ = ([(n, _I32) for n in ("positions", "channels", "method", "reserved")]
+                + [(n, ctypes.c_double) for n in ("start", "theta", "factor", "original")])
+
+
+class VsaRotaryOp(ctypes.Structure):
+    """``struct vsa_rotary_op`` of the header."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "q_out", "k_out", "cos", "sin", "positions")]
+                + [(n, _I64 * 3) for n in ("q_stride", "k_stride", "q_out_stride",
+                                           "k_out_stride")]
+                + [(n, _I64) for n in ("positions_stride", "batch", "tokens", "rows")]
+                + [(n, _I32) for n in ("q_heads", "k_heads", "head_dim", "channels",
+                                       "interleaved", "inverse", "positions64", "dtype")])
+
+
+class VsaCross(ctypes.Structure):
+    """``struct vsa_cross`` of the header."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "kv_lens", "key_mask")]
+                + [(n, _I64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [(n, _I64) for n in ("mask_stride", "sq", "skv")]
+                + [(n, _I32) for n in ("batch", "heads", "kv_heads", "head_dim", "dtype")]
                 + [("scale", _F)])
 
 

@@ -1,0 +1,193 @@
+"""Cross attention of video tokens to an encoder's states on MI355X: queries of
+one length, keys and values of another, each sample with its own valid keys.
+
+    out = softmax(sm_scale * q k^T over the sample's valid keys) v
+
+The forward and the backward are one call each into the C ABI
+(``vsa_cross_fwd`` / ``vsa_cross_bwd``), on torch's current stream, with a
+workspace from torch's allocator.  Nothing here runs on the CPU: a CPU tensor or
+a missing kernel library raises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+from typing import Optional
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .launch import _ptr, _workspace, on_device
+from .mi355x import KERNEL_DTYPES, _i32
+from .rotary import empty_in_order, strides
+
+MAX_HEAD_DIM = 256
+MAX_TOKENS = (1 << 31) - 256
+
+
+def _rows16(x: Tensor) -> Tensor:
+    """x itself where the kernels read its rows in place (channels next to each
+    other, every row 16-byte aligned, a tile's rows within reach of a 32-bit
+    offset), else a dense copy."""
+    es = x.element_size()
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0:
+        st = [n for n, size in zip(x.stride()[:3], x.shape[:3]) if size > 1]
+        if all(n * es % 16 == 0 for n in st) and \
+                (x.shape[2] == 1 or x.stride(2) <= (1 << 30) // (64 * es)):
+            return x
+    return x.clone() if x.is_contiguous() else x.contiguous()
+
+
+def _struct(q, k, v, lens, mask, scale) -> _lib.VsaCross:
+    return _lib.VsaCross(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lens), _ptr(mask), strides(q), strides(k),
+        strides(v), 0 if mask is None else mask.stride(0), q.shape[2], k.shape[2], q.shape[0],
+        q.shape[1], k.shape[1], q.shape[3], _lib.dtype_code(q.dtype), scale)
+
+
+@functools.lru_cache(maxsize=256)
+def _sizes(b, h, hk, sq, skv, d, masked, dtype):
+    """Bytes of (forward scratch, backward scratch)."""
+    some, zero = 256, (ctypes.c_int64 * 3)()   # any aligned pointer: only its presence is read
+    c = _lib.VsaCross(some, some, some, None, some if masked else None, zero, zero, zero, 0, sq,
+                      skv, b, h, hk, d, dtype, 1.0)
+    n = (ctypes.c_int64 * 2)()
+    at = ctypes.addressof(n)
+    _lib.call("vsa_cross_sizes", ctypes.addressof(c), at, at + 8)
+    return tuple(n)
+
+
+def _scratch(c: _lib.VsaCross, masked: bool, which: int, device) -> Optional[Tensor]:
+    return _workspace(_sizes(c.batch, c.heads, c.kv_heads, c.sq, c.skv, c.head_dim, masked,
+                             c.dtype)[which], device)
+
+
+def _forward(q, k, v, lens, mask, scale, keep):
+    """(out, lo, lse); the last two only where the backward needs them (``keep``)."""
+    dev = q.device
+    with on_device(dev):
+        c = _struct(q, k, v, lens, mask, scale)
+        out = empty_in_order(q)
+        lo = lse = None
+        if keep:
+            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
+            if q.dtype != torch.float32:
+                lo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        scratch, st = _scratch(c, mask is not None, 0, dev), strides(out)
+        _lib.call("vsa_cross_fwd", ctypes.addressof(c), out.data_ptr(), ctypes.addressof(st),
+                  _ptr(lo), _ptr(lse), _ptr(scratch),
+                  torch._C._cuda_getCurrentRawStream(dev.index))
+    return out, lo, lse
+
+
+def _backward(q, k, v, lens, mask, scale, out, lo, lse, dout):
+    dev = q.device
+    with on_device(dev):
+        # (the saved ones too: a saved-tensor hook may give back other addresses)
+        q, k, v, out, dout = (_rows16(x) for x in (q, k, v, out, dout))
+        lo = lo if lo is None else _rows16(lo.contiguous())
+        c = _struct(q, k, v, lens, mask, scale)
+        dq, dk, dv = (empty_in_order(x) for x in (q, k, v))
+        scratch = _scratch(c, mask is not None, 1, dev)
+        s = [strides(x) for x in (out, dout, dq, dk, dv)]
+        at = [ctypes.addressof(x) for x in s]
+        _lib.call("vsa_cross_bwd", ctypes.addressof(c), out.data_ptr(), at[0], _ptr(lo),
+                  dout.data_ptr(), at[1], lse.data_ptr(), dq.data_ptr(), at[2], dk.data_ptr(), at[3],
+                  dv.data_ptr(), at[4], _ptr(scratch),
+                  torch._C._cuda_getCurrentRawStream(dev.index))
+    return dq, dk, dv
+
+
+class _Cross(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lens, mask, scale):
+        out, lo, lse = _forward(q, k, v, lens, mask, scale, True)
+        ctx.save_for_backward(q, k, v, lens, mask, out, lo, lse)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, lens, mask, out, lo, lse = ctx.saved_tensors
+        return (*_backward(q, k, v, lens, mask, ctx.scale, out, lo, lse, dout), None, None, None)
+
+
+def _check(q, k, v, kv_lens, key_mask, sm_scale) -> None:
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
+        raise ValueError("q, k, and v must have shape [batch, heads, seq_len, dim]")
+    b, h, sq, d = q.shape
+    if k.shape[0] != b or v.shape[0] != b:
+        raise ValueError("q, k, and v must share the batch dimension")
+    if v.shape[1] != k.shape[1] or v.shape[2] != k.shape[2]:
+        raise ValueError("k and v must have the same heads and sequence length")
+    if k.shape[3] != d or v.shape[3] != d:
+        raise ValueError("q, k, and v must have the same head dimension")
+    if (h and not k.shape[1]) or (k.shape[1] and h % k.shape[1]):
+        raise ValueError(f"the {h} heads of q must be a multiple of the {k.shape[1]} of k and v")
+    if not q.dtype == k.dtype == v.dtype:
+        raise ValueError("q, k, and v must have the same dtype")
+    if q.dtype not in KERNEL_DTYPES:
+        raise ValueError("the MI355X kernels support float16, bfloat16 and float32")
+    if not 1 <= d <= MAX_HEAD_DIM:
+        raise ValueError(f"the MI355X kernels support head_dim <= {MAX_HEAD_DIM}")
+    if kv_lens is not None:
+        if tuple(kv_lens.shape) != (b,):
+            raise ValueError("kv_lens must have shape [batch]")
+        if kv_lens.dtype not in (torch.int32, torch.int64):
+            raise ValueError("kv_lens must be int32 or int64")
+    if key_mask is not None:
+        if tuple(key_mask.shape) != (b, k.shape[2]):
+            raise ValueError("key_mask must have shape [batch, kv seq_len]")
+        if key_mask.dtype != torch.bool:
+            raise ValueError("key_mask must be bool (True: the key is attended to)")
+    if sm_scale is not None and not math.isfinite(sm_scale):
+        raise ValueError("sm_scale must be finite")
+    if b > 65535 or h > 65535 or k.shape[2] > MAX_TOKENS or \
+            (h and sq > MAX_TOKENS // (h // k.shape[1])):
+        raise ValueError("the MI355X kernels support at most 65535 samples and heads, and fewer "
+                         "than 2^31 query rows of a key head and keys")
+    tensors = [x for x in (q, k, v, kv_lens, key_mask) if x is not None]
+    if not all(x.is_cuda for x in tensors):
+        raise ValueError("the MI355X implementation requires GPU tensors")
+    if any(x.device != q.device for x in tensors):
+        raise ValueError("q, k, v, kv_lens and key_mask must be on the same GPU device")
+
+
+def mi355x_cross_attention(q: Tensor, k: Tensor, v: Tensor, kv_lens: Optional[Tensor] = None,
+                           key_mask: Optional[Tensor] = None, *,
+                           sm_scale: Optional[float] = None) -> Tensor:
+    """Attention of ``q`` ``[batch, heads, seq_len, dim]`` to an encoder's ``k``, ``v``
+    ``[batch, kv_heads, kv_len, dim]`` (``heads`` a multiple of ``kv_heads``; any
+    lengths), over the keys below ``kv_lens[b]`` (clamped to ``[0, kv_len]``) whose
+    ``key_mask[b]`` is True.  A sample without a valid key gets zeros; what lies
+    behind a masked key (NaN included) has no influence.  ``sm_scale`` defaults to
+    ``1/sqrt(dim)``.
+
+    Per-head views of token-major memory, slices of a packed projection and
+    expanded (broadcast) tensors are read in place where their rows start 16-byte
+    aligned; the result is dense, in q's order of heads and tokens.
+    Differentiable once in q, k and v."""
+    _check(q, k, v, kv_lens, key_mask, sm_scale)
+    d = q.shape[3]
+    if q.numel() == 0 or k.numel() == 0:
+        # nothing to attend with or to: zeros, in the graph of every input
+        rest = sum(x[..., :0].sum() for x in (q, k, v))
+        return torch.zeros(q.shape, dtype=q.dtype, device=q.device) + rest
+    scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d)
+    lens = None if kv_lens is None else _i32(kv_lens, q.device)
+    mask = key_mask
+    if mask is not None and mask.stride(1) != 1 and mask.shape[1] > 1:
+        mask = mask.contiguous()
+    if d % 8:   # rows of whole 16-byte pieces; zero channels change no product
+        q, k, v = (torch.nn.functional.pad(x, (0, 8 - d % 8)) for x in (q, k, v))
+    q, k, v = (_rows16(x) for x in (q, k, v))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out = _Cross.apply(q, k, v, lens, mask, scale)
+    else:
+        out = _forward(q, k, v, lens, mask, scale, False)[0]
+    return out[..., :d] if d % 8 else out

@@ -1,0 +1,232 @@
+"""Rotary positions of video tokens on MI355X: a latent grid's table and the
+rotation of q and k by it, before the attention.
+
+A pair of channels at angle a becomes (x1 cos a - x2 sin a, x2 cos a + x1 sin a);
+the angle is the token's position along an axis of the grid times the pair's
+frequency.  Both are HIP kernels (``vsa_rotary_table``, ``vsa_rotary``); the
+rotation is differentiable to any order (its gradient is the opposite rotation).
+Nothing here runs on the CPU: a CPU tensor or a missing kernel library raises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .launch import on_device
+
+ROTARY_METHODS = ("linear", "ntk", "yarn")
+MAX_ROTARY_CHANNELS = 256
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+# ---------------------------------------------------------------------------
+# Table
+# ---------------------------------------------------------------------------
+
+def _three(x, name, kind=float) -> Tuple:
+    x = tuple(x) if isinstance(x, (tuple, list)) else (x,) * 3
+    if len(x) != 3:
+        raise ValueError(f"{name} must have three entries (T, H, W)")
+    return tuple(kind(v) for v in x)
+
+
+def build_rotary_table(dit_seq_shape: Tuple[int, int, int], axis_channels: Tuple[int, int, int],
+                       theta: float = 10000.0, *, start=(0, 0, 0),
+                       factor: Union[float, Tuple[float, float, float]] = 1.0,
+                       method: str = "linear", original_shape=None,
+                       device: torch.device | str = "cuda") -> Tuple[Tensor, Tensor]:
+    """``(cos, sin)``, fp32 ``[T*H*W, sum(axis_channels) / 2]``, of the raster-order
+    tokens of a ``(T, H, W)`` grid: pair i of an axis with d channels turns by
+    ``(start + index) * theta ** (-2 i / d)``.  A plain sequence is ``(S, 1, 1)``
+    with ``(channels, 0, 0)``.
+
+    ``method`` scales the axes for grids longer than a model was trained on, by
+    ``factor`` (one number or one an axis): "linear" divides the positions,
+    "ntk" takes ``theta * factor ** (d / (d - 2))``, "yarn" keeps the frequencies
+    that turn 32 times or more in ``original_shape`` (the trained sizes), divides
+    those that turn once or less, a ramp between, and multiplies cos and sin by
+    ``0.1 ln(factor) + 1``.  Angles are made in 64 bits."""
+    shape = _three(dit_seq_shape, "dit_seq_shape", int)
+    channels = _three(axis_channels, "axis_channels", int)
+    start, factor = _three(start, "start"), _three(factor, "factor")
+    if min(shape) <= 0:
+        raise ValueError("dit_seq_shape must be positive")
+    if math.prod(shape) >= 1 << 31:
+        raise ValueError("a rotary table holds fewer than 2^31 tokens")
+    if min(channels) < 0 or any(c % 2 for c in channels) or not \
+            0 < sum(channels) <= MAX_ROTARY_CHANNELS:
+        raise ValueError("axis_channels must be even, and together in "
+                         f"[2, {MAX_ROTARY_CHANNELS}]")
+    theta = float(theta)
+    if not (theta > 0 and math.isfinite(theta)):
+        raise ValueError("theta must be positive and finite")
+    if not all(f > 0 and math.isfinite(f) for f in factor):
+        raise ValueError("factor must be positive and finite")
+    if not all(abs(x) <= 2.0 ** 52 for x in start):
+        raise ValueError("start must lie within 2^52")
+    if method not in ROTARY_METHODS:
+        raise ValueError(f"method must be one of {ROTARY_METHODS}")
+    original = (0.0,) * 3
+    if method == "yarn":
+        if original_shape is None:
+            raise ValueError("the yarn method needs original_shape, the trained (T, H, W)")
+        original = _three(original_shape, "original_shape")
+        if not all(x > 0 and math.isfinite(x) for x in original):
+            raise ValueError("original_shape must be positive")
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError("the MI355X implementation requires a GPU device")
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    axes = (_lib.VsaRotaryAxis * 3)(*(
+        _lib.VsaRotaryAxis(shape[i], channels[i], ROTARY_METHODS.index(method), 0, start[i], theta,
+                           factor[i], original[i]) for i in range(3)))
+    cos = torch.empty((math.prod(shape), sum(channels) // 2), dtype=torch.float32, device=device)
+    sin = torch.empty_like(cos)
+    with on_device(device):
+        _lib.call("vsa_rotary_table", ctypes.addressof(axes), cos.data_ptr(), sin.data_ptr(),
+                  torch._C._cuda_getCurrentRawStream(device.index))
+    return cos, sin
+
+
+# ---------------------------------------------------------------------------
+# Rotation
+# ---------------------------------------------------------------------------
+
+def token_order(x: Tensor) -> bool:
+    """True for a [B, H, S, D] tensor whose heads lie closer together than its
+    tokens (a per-head view of token-major memory)."""
+    return x.shape[1] > 1 and x.shape[2] > 1 and x.stride(1) < x.stride(2)
+
+
+def empty_in_order(x: Tensor, shape=None) -> Tensor:
+    """An uninitialised [B, H, S, D] tensor, dense, in x's order of heads and tokens."""
+    b, h, s, d = x.shape if shape is None else shape
+    if token_order(x):
+        return torch.empty((b, s, h, d), dtype=x.dtype, device=x.device).transpose(1, 2)
+    return torch.empty((b, h, s, d), dtype=x.dtype, device=x.device)
+
+
+def strides(x: Tensor):
+    """Strides of batch, head and token for the C ABI; 0 for a dimension of one."""
+    return (ctypes.c_int64 * 3)(*(n if size > 1 else 0
+                                  for n, size in zip(x.stride(), x.shape[:3])))
+
+
+def _rotate(q, k, cos, sin, positions, interleaved, inverse):
+    """One launch: (q turned, k turned); k may be None."""
+    q, k = (x if x is None or x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+            for x in (q, k))
+    q_out, k_out = empty_in_order(q), None if k is None else empty_in_order(k)
+    b, h, s, d = q.shape
+    kk, ko = (q, q_out) if k is None else (k, k_out)
+    op = _lib.VsaRotaryOp(
+        q.data_ptr(), kk.data_ptr(), q_out.data_ptr(), ko.data_ptr(), cos.data_ptr(),
+        sin.data_ptr(), None if positions is None else positions.data_ptr(), strides(q),
+        strides(kk), strides(q_out), strides(ko),
+        0 if positions is None or positions.dim() == 1 else s, b, s, cos.shape[0], h,
+        0 if k is None else k.shape[1], d, 2 * cos.shape[1], interleaved, inverse,
+        positions is not None and positions.dtype is torch.int64, _lib.dtype_code(q.dtype))
+    with on_device(q.device):
+        _lib.call("vsa_rotary", ctypes.addressof(op),
+                  torch._C._cuda_getCurrentRawStream(q.device.index))
+    return q_out, k_out
+
+
+class _Rotary(torch.autograd.Function):
+    """Its gradient is itself, turned the other way."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.options = interleaved, inverse
+        return _rotate(q, k, cos, sin, positions, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        cos, sin, positions = ctx.saved_tensors
+        interleaved, inverse = ctx.options
+        got = [g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad)]
+        live = [g for g in got if g is not None]
+        if live:
+            rest = (cos, sin, positions, interleaved, not inverse)
+            turned = iter(_Rotary.apply(live[0], live[1] if len(live) > 1 else None, *rest))
+            got = [None if g is None else next(turned) for g in got]
+        return (*got, None, None, None, None, None)
+
+
+def _check_rotary(q, k, cos, sin, positions) -> None:
+    if q.ndim != 4 or (k is not None and k.ndim != 4):
+        raise ValueError("q and k must have shape [batch, heads, seq_len, dim]")
+    b, _, s, d = q.shape
+    if k is not None:
+        if k.shape[0] != b or k.shape[2] != s or k.shape[3] != d:
+            raise ValueError("q and k must share batch, sequence length and head dimension")
+        if k.dtype != q.dtype:
+            raise ValueError("q and k must have the same dtype")
+    if q.dtype not in _DTYPES:
+        raise ValueError("the MI355X kernels support float16, bfloat16 and float32")
+    if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or \
+            sin.dtype != torch.float32:
+        raise ValueError("cos and sin must be float32 tensors of one shape [positions, channels / 2]")
+    if not 2 <= 2 * cos.shape[1] <= d:
+        raise ValueError(f"the table turns {2 * cos.shape[1]} channels of a head of {d}")
+    if d > 256:
+        raise ValueError("the MI355X kernels support head_dim <= 256")
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError("cos and sin get no gradient: detach them")
+    if positions is None:
+        if cos.shape[0] < s:
+            raise ValueError(f"the table has {cos.shape[0]} positions for {s} tokens")
+    else:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError("positions must be int32 or int64")
+        if tuple(positions.shape) not in ((s,), (b, s)):
+            raise ValueError("positions must have shape [seq_len] or [batch, seq_len]")
+        if cos.shape[0] == 0:
+            raise ValueError("the table has no positions")
+    tensors = [x for x in (q, k, cos, sin, positions) if x is not None]
+    if not all(x.is_cuda for x in tensors):
+        raise ValueError("the MI355X implementation requires GPU tensors")
+    if any(x.device != q.device for x in tensors):
+        raise ValueError("q, k, the table and the positions must be on the same GPU device")
+
+
+def mi355x_rotary(q: Tensor, k: Optional[Tensor], cos: Tensor, sin: Tensor,
+                  positions: Optional[Tensor] = None, *, interleaved: bool = False,
+                  inverse: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+    """``(q, k)`` turned by their positions: ``[batch, heads, seq_len, dim]`` (their
+    head counts may differ; ``k`` may be None), the first ``2 * cos.shape[1]``
+    channels of each head, in pairs ``(i, i + n/2)`` or, with ``interleaved``,
+    ``(2i, 2i + 1)``; the other channels are copied.  ``inverse`` turns back.
+
+    Token s takes row s of the table ``cos``, ``sin`` (``build_rotary_table``), or
+    row ``positions[s]`` / ``positions[b, s]``; a negative position copies the
+    token (a padding slot of ``slot_rows``), one past the table gives NaN.
+
+    Per-head views of token-major memory and slices of a packed projection are
+    read in place; the results are dense, in the order of heads and tokens of
+    the input.  Differentiable in q and k to any order."""
+    _check_rotary(q, k, cos, sin, positions)
+    cos, sin = cos.contiguous(), sin.contiguous()
+    if positions is not None:
+        positions = positions.contiguous()
+    interleaved, inverse = bool(interleaved), bool(inverse)
+    if k is not None and k.shape[1] == 0:
+        return mi355x_rotary(q, None, cos, sin, positions, interleaved=interleaved,
+                             inverse=inverse)[0], k * 1
+    if q.numel() == 0:
+        if k is not None and k.numel():
+            return q * 1, mi355x_rotary(k, None, cos, sin, positions, interleaved=interleaved,
+                                        inverse=inverse)[0]
+        return q * 1, None if k is None else k * 1
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, cos, sin, positions, interleaved, inverse)
+    return _rotate(q, k, cos, sin, positions, interleaved, inverse)

@@ -36,6 +36,7 @@ from torch import Tensor
 from . import _lib, launch
 from . import mi355x as M
 from . import tiling
+from .rotary import _check_rotary, mi355x_rotary
 
 FUSED_BLOCKS = (64, 128, 256)
 FUSED_HEAD_DIMS = (64, 128)
@@ -129,10 +130,20 @@ def _composition(q, k, v, meta, nb, be, tile_size, topk, gate, token_major=False
     return tiling.untile(out.reshape(b * h, nb * be, d), npi, rev).view(b, h, -1, d)
 
 
+def _rotated(q, k, rotary, interleaved, token_major):
+    """q and k turned by a table of the grid's raster tokens."""
+    if token_major:
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
+    q, k = mi355x_rotary(q, k, *rotary, interleaved=interleaved)
+    return (q.transpose(1, 2), k.transpose(1, 2)) if token_major else (q, k)
+
+
 def mi355x_vsa_tiled(q: Tensor, k: Tensor, v: Tensor, dit_seq_shape: Tuple[int, int, int],
                      topk: int, tile_size: Tuple[int, int, int] = tiling.VSA_TILE_SIZE,
                      compress_attn_weight: Optional[Tensor] = None,
-                     token_major: bool = False) -> Tensor:
+                     token_major: bool = False,
+                     rotary: Optional[Tuple[Tensor, Tensor]] = None,
+                     rotary_interleaved: bool = False) -> Tensor:
     """VSA on raster-order tokens of a ``(T, H, W)`` latent grid: ``[B, H,
     T*H*W, D]``, or ``[B, T*H*W, H, D]`` with ``token_major`` (the gate and the
     result in the same layout).
@@ -141,7 +152,11 @@ def mi355x_vsa_tiled(q: Tensor, k: Tensor, v: Tensor, dit_seq_shape: Tuple[int, 
     tile_size, tile(gate)))`` with tile / untile along the sequence dim and
     ``vbs`` the tiles' real-token counts (build_vsa_metadata), bit for bit;
     the tile and untile passes (fastvideo_tiling.py:130-145) are fused into
-    the op's own passes."""
+    the op's own passes.
+
+    ``rotary``: the grid's ``(cos, sin)`` (``build_rotary_table``); q and k are
+    turned by it first, as ``mi355x_rotary`` turns them (``rotary_interleaved``
+    its pairing)."""
     if q.dim() != 4 or k.shape != q.shape or v.shape != q.shape:
         raise ValueError("mi355x_vsa_tiled expects q, k, v of one shape [batch, heads, seq_len, "
                          "head_dim] ([batch, seq_len, heads, head_dim] with token_major) "
@@ -163,8 +178,12 @@ def mi355x_vsa_tiled(q: Tensor, k: Tensor, v: Tensor, dit_seq_shape: Tuple[int, 
     # the checks read [B, H, S, D] shapes: token-major tensors as head-major views
     M._check_device_path(*(x.transpose(1, 2) if token_major else x for x in (q, k, v)), be)
     M._check_block_count(nb, q)
+    if rotary is not None:
+        _check_rotary(q.transpose(1, 2) if token_major else q, None, *rotary, None)
     if q.shape[0] * (q.shape[2] if token_major else q.shape[1]) == 0:
         return M._empty_batch(q, k, v, compress_attn_weight)
+    if rotary is not None:
+        q, k = _rotated(q, k, rotary, rotary_interleaved, token_major)
     gate = compress_attn_weight
     b, h, _, d = _dims(q, token_major)
     full, per_token = ((b, s_out, h, d), (b, s_out, h, 1)) if token_major else \

@@ -1,0 +1,107 @@
+"""What the cross attention refuses, before anything reaches a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+from vsa_mi355x import _lib, mi355x_cross_attention
+
+
+def _args(**kw):
+    a = dict(q=torch.zeros(2, 4, 5, 64), k=torch.zeros(2, 2, 7, 64), v=torch.zeros(2, 2, 7, 64),
+             kv_lens=None, key_mask=None)
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(q=torch.zeros(4, 5, 64)), "batch, heads"),
+    (dict(q=torch.zeros(3, 4, 5, 64)), "batch"),
+    (dict(v=torch.zeros(2, 1, 7, 64)), "same heads"),
+    (dict(v=torch.zeros(2, 2, 6, 64)), "sequence length"),
+    (dict(q=torch.zeros(2, 4, 5, 32)), "head dimension"),
+    (dict(q=torch.zeros(2, 3, 5, 64)), "multiple"),
+    (dict(k=torch.zeros(2, 0, 7, 64), v=torch.zeros(2, 0, 7, 64)), "multiple"),
+    (dict(k=torch.zeros(2, 2, 7, 64).half()), "same dtype"),
+    (dict(q=torch.zeros(2, 4, 5, 64).double(), k=torch.zeros(2, 2, 7, 64).double(),
+          v=torch.zeros(2, 2, 7, 64).double()), "float16"),
+    (dict(q=torch.zeros(2, 4, 5, 264), k=torch.zeros(2, 2, 7, 264),
+          v=torch.zeros(2, 2, 7, 264)), "256"),
+    (dict(kv_lens=torch.zeros(3, dtype=torch.int32)), "kv_lens"),
+    (dict(kv_lens=torch.zeros(2)), "int32"),
+    (dict(key_mask=torch.ones(2, 8, dtype=torch.bool)), "key_mask"),
+    (dict(key_mask=torch.ones(2, 7)), "bool"),
+    (dict(sm_scale=float("nan")), "finite"),
+    (dict(sm_scale=float("inf")), "finite"),
+    ({}, "GPU"),
+])
+def test_refusals(kw, text):
+    with pytest.raises(ValueError, match=text):
+        mi355x_cross_attention(**_args(**kw))
+
+
+def test_entry_points_refuse_without_a_launch():
+    lib = _lib.load()
+    buf = torch.zeros(256)
+    p = (buf.data_ptr() + 255) // 256 * 256
+    st = (ctypes.c_int64 * 3)(64, 64, 64)
+    n = (ctypes.c_int64 * 2)()
+    at = ctypes.addressof(n)
+    s3 = ctypes.addressof(st)
+
+    def struct(**kw):
+        c = _lib.VsaCross()
+        c.q = c.k = c.v = p
+        c.q_stride[:] = c.k_stride[:] = c.v_stride[:] = [64, 64, 64]
+        c.sq, c.skv, c.batch, c.heads, c.kv_heads, c.head_dim = 4, 6, 2, 4, 2, 64
+        c.scale = 0.125
+        for name, x in kw.items():
+            if name.endswith("stride") and name != "mask_stride":
+                getattr(c, name)[:] = x
+            else:
+                setattr(c, name, x)
+        return c
+
+    def sizes(**kw):
+        c = struct(**kw)
+        return lib.vsa_cross_sizes(ctypes.addressof(c), at, at + 8)
+
+    assert sizes() == 0 and n[0] >= 0 and n[1] > 0
+    assert sizes(q=None) == -1 and sizes(dtype=9) == -3
+    for kw in (dict(batch=0), dict(heads=3), dict(kv_heads=0), dict(head_dim=60),
+               dict(head_dim=264), dict(sq=0), dict(skv=0), dict(skv=1 << 31), dict(sq=1 << 31),
+               dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=65536)):
+        assert sizes(**kw) == -2, kw
+    assert sizes(k=p + 8) == -7 and sizes(v_stride=[64, 64, 4]) == -7
+    assert sizes(q_stride=[-64, 64, 64]) == -7 and sizes(k_stride=[64, 64, 1 << 30]) == -7
+    assert sizes(kv_lens=p + 2) == -7
+    c = struct()
+    assert lib.vsa_cross_fwd(ctypes.addressof(c), None, s3, None, None, None, None) == -1
+    assert lib.vsa_cross_fwd(ctypes.addressof(c), p + 2, s3, None, None, None, None) == -7
+    c = struct(key_mask=p)
+    assert lib.vsa_cross_fwd(ctypes.addressof(c), p, s3, None, None, None, None) == -1   # no scratch
+    c = struct()
+    bwd = [ctypes.addressof(c), p, s3, None, p, s3, p, p, s3, p, s3, p, s3, p, None]
+    for i in (1, 2, 4, 6, 7, 9, 11, 13):
+        bad = list(bwd)
+        bad[i] = None
+        assert lib.vsa_cross_bwd(*bad) == -1, i
+    bwd[9] = p + 4
+    assert lib.vsa_cross_bwd(*bwd) == -7
+
+
+def test_workspaces_are_bounded():
+    """The parts of a split never exceed what one row of workgroups can fill: the
+    forward's scratch at a few queries on a long context, and the backward's at a
+    long video on a prompt."""
+    lib = _lib.load()
+    n = (ctypes.c_int64 * 2)()
+    at = ctypes.addressof(n)
+    for b, h, sq, skv, d in ((1, 12, 64, 40960, 128), (8, 12, 1, 512, 128),
+                             (1, 40, 40960, 512, 128), (1, 1, 1, 1 << 20, 64)):
+        c = _lib.VsaCross()
+        c.q = c.k = c.v = 256
+        c.sq, c.skv, c.batch, c.heads, c.kv_heads, c.head_dim, c.scale = sq, skv, b, h, h, d, 1.0
+        assert lib.vsa_cross_sizes(ctypes.addressof(c), at, at + 8) == 0
+        assert n[0] <= 1 << 28 and n[1] <= 1 << 30, (n[0], n[1])

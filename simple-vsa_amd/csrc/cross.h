@@ -7,10 +7,10 @@
 // a group (heads / kv_heads) share a key head.  A key is valid if it lies below
 // its sample's kv_lens and its key_mask byte is not zero.
 //
-// Tiles of K and V (or Q and dO) are copied to LDS by direct loads; the rows of
-// keys that are not valid, and the channels past the head dim, are fetched from
-// 16 bytes of zeros instead, so that nothing behind a mask (infinities, NaN,
-// memory past the last row) takes part in a product.
+// Tiles of K and V (or Q and dO) are copied to LDS by direct loads that write
+// zeros for the rows of keys that are not valid and for the channels past the
+// head dim, so that nothing behind a mask (infinities, NaN, memory past the last
+// row) takes part in a product.
 #pragma once
 
 #include "vsa_device.h"
@@ -68,12 +68,14 @@ __device__ __forceinline__ typename Mma<T>::V8 zero8() {
   return z;
 }
 
-// fp32 at head dim 256 leaves no registers to read operands ahead: without a
-// fence after each step of a product the compiler moves the reads of all of
-// them to the front and spills.
+// Wide rows leave no registers to read many operands ahead: without a fence after
+// each step of a product the compiler moves the reads of all of them to the
+// front and spills (head dim 256, and 128 in fp32).
+template <typename T, int D>
+constexpr bool kWide = D * sizeof(T) > 256;
 template <typename T, int D>
 __device__ __forceinline__ void step_fence() {
-  if constexpr (D * sizeof(T) > 512) __builtin_amdgcn_sched_barrier(0);
+  if constexpr (kWide<T, D>) __builtin_amdgcn_sched_barrier(0);
 }
 
 // LDS tile of rows of D elements, 16-byte chunks swizzled by the row: 16-bit
@@ -135,70 +137,156 @@ __device__ __forceinline__ typename Mma<T>::V8 col_op(const char* X, int d0, int
   }
 }
 
-// What copies of masked rows and of channels past the head dim read, and what
-// the statistics of query rows past the last one read: P = 2^(s - inf) = 0.
-__device__ __attribute__((aligned(16))) static const uint32_t kZero16[4] = {0, 0, 0, 0};
+// What the statistics of query rows past the last one read: P = 2^(s - inf) = 0.
 __device__ __attribute__((aligned(16))) static const float kPastStats[2] = {INFINITY, 0.f};
 
-// Copies ROWS rows of D elements into a tile, as NT threads.  Rows whose bit of
-// `valid` is clear become zeros, and so do channels past `dim`.  The byte
-// offsets of a thread's pieces are kept in registers where there are up to
-// eight of them; more are worked out again for each copy.
+// Direct copies of 16 bytes a lane to LDS through a buffer descriptor: a lane
+// whose offset lies past the descriptor's bytes writes zeros, so rows past the
+// last one, keys behind a mask and channels past the head dim need no branch
+// and no address of their own (dma16 in vsa_device.h explains the asm's form).
+typedef u32x4 Srd;
+__device__ __forceinline__ Srd srd_of(const void* base, uint32_t bytes) {
+  // (uniform values, in scalar registers whatever the compiler knows of them)
+  const uint64_t p = (uint64_t)(uintptr_t)base;
+  return Srd{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p),
+             (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32)) & 0xffffu,
+             (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
+__device__ __forceinline__ void dma16_b(uint32_t voff, Srd srd, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff),
+               "s"(srd), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+constexpr uint32_t kPastEnd = 0x80000000u;  // descriptors hold less than 2^31 bytes
+
+// Copies ROWS rows of D elements into a tile, as threads 0 .. NT - 1 (whole waves
+// of a workgroup).  A thread keeps the
+// byte offsets of up to eight of its 16-byte pieces; the swizzle repeats every
+// 16 rows, so the pieces of later rows take the same offsets from a descriptor
+// that starts 16 rows on.
 template <typename T, int D, int ROWS, int NT>
 struct TileCopy {
   typedef Tile<T, D> L;
-  static constexpr int N = ROWS * L::CH / NT;  // 16-byte pieces of a thread
-  static constexpr bool KEEP = N <= 8;
-  static_assert(ROWS * L::CH % NT == 0 && ROWS % 32 == 0, "");
-  uint32_t voff[KEEP ? N : 1];   // byte offset of the piece from the tile's first row
+  static constexpr int N = ROWS * L::CH / NT;                   // pieces of a thread
+  static constexpr int K = N <= 8 ? N : 16 * L::CH / NT;        // of them kept
+  static constexpr int G = N / K;                               // descriptors
+  static constexpr bool KEEP = D * sizeof(T) <= 512;            // else worked out again
+  static_assert(ROWS * L::CH % NT == 0 && ROWS % 32 == 0 && N % K == 0 && K <= 8, "");
+  uint32_t voff[KEEP ? K : 1];   // byte offset of the piece from the descriptor's first row
   uint32_t stride;               // bytes between rows
   int dim;                       // bytes of a row
+  uint32_t wave;                 // of this thread's wave, bytes into each piece
+  int tid;
+  struct Src {
+    Srd s[G];
+  };
 
-  static __device__ __forceinline__ int place(int i, int tid, int& c) {
-    return L::unoff(i * NT + tid, c);
-  }
-  __device__ __forceinline__ uint32_t offset(int i, int tid) const {
-    int c;
-    const int row = place(i, tid, c);
-    return (uint32_t)row * stride + (uint32_t)c * 16u;
-  }
-  __device__ __forceinline__ void init(int64_t row_stride, int channels) {
+  __device__ __forceinline__ void init(int64_t row_stride, int channels, int thread) {
     stride = (uint32_t)(row_stride * (int)sizeof(T));
     dim = channels * (int)sizeof(T);
+    tid = thread;
+    wave = (uint32_t)__builtin_amdgcn_readfirstlane(thread >> 6) * 1024u;
     if constexpr (KEEP) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) voff[i] = opaque(offset(i, threadIdx.x));
+      for (int i = 0; i < K; ++i) voff[i] = opaque(offset(i, tid));
     }
   }
-  static __device__ __forceinline__ uint32_t lds_base(uint32_t lds) {
-    return lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024u;
+  __device__ __forceinline__ uint32_t offset(int i, int t) const {
+    int c;
+    const int row = L::unoff(i * NT + t, c);
+    return c * 16 < dim ? (uint32_t)row * stride + (uint32_t)c * 16u : kPastEnd;
   }
-  // every row valid, every channel within the head dim
-  __device__ __forceinline__ void whole(uint32_t lds, const T* src) const {
-    const uint32_t base = lds_base(lds);
-    const int tid = KEEP ? 0 : opaque((int)threadIdx.x);
+  __device__ __forceinline__ uint32_t at(int i) const {
+    return KEEP ? voff[KEEP ? i % K : 0] : offset(i % K, opaque(tid));
+  }
+  // the rows from src on, `left` (>= 1) of which exist
+  __device__ __forceinline__ Src rows(const T* src, int left) const {
+    Src r;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      dma16_s(KEEP ? voff[KEEP ? i : 0] : offset(i, tid), src, base + (uint32_t)i * (NT / 64) * 1024u);
+    for (int g = 0; g < G; ++g) {
+      const int n = min(left, ROWS) - 16 * g;
+      r.s[g] = srd_of(reinterpret_cast<const char*>(src) + (uint64_t)(16 * g) * stride,
+                      n > 0 ? (uint32_t)(n - 1) * stride + (uint32_t)dim : 0u);
+    }
+    return r;
   }
-  __device__ __forceinline__ void part(uint32_t lds, const T* src,
-                                       const uint32_t (&valid)[ROWS / 32]) const {
-    const uint32_t base = lds_base(lds);
-    const int tid = opaque((int)threadIdx.x);
+  __device__ __forceinline__ void piece(int i, uint32_t lds, const Src& src) const {
+    dma16_b(at(i), src.s[i / K], lds + wave + (uint32_t)i * (NT / 64) * 1024u);
+  }
+  __device__ __forceinline__ void copy(uint32_t lds, const Src& src) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) piece(i, lds, src);
+  }
+  // Rows whose bit of `valid` is clear become zeros.
+  __device__ __forceinline__ void copy_valid(uint32_t lds, const Src& src,
+                                             const uint32_t (&valid)[ROWS / 32]) const {
+    const int t = opaque(tid);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       int c;
-      const int row = place(i, tid, c);
+      const int row = L::unoff(i * NT + t, c);
       uint32_t w = valid[0];
 #pragma unroll
       for (int x = 1; x < ROWS / 32; ++x) w = row >= 32 * x ? valid[x] : w;
-      const bool on = ((w >> (row & 31)) & 1u) != 0 && c * 16 < dim;
-      const char* g = on ? reinterpret_cast<const char*>(src) + offset(i, tid)
-                         : reinterpret_cast<const char*>(kZero16);
-      dma16(g, base + (uint32_t)i * (NT / 64) * 1024u);
+      dma16_b((w >> (row & 31)) & 1u ? at(i) : kPastEnd, src.s[i / K],
+              lds + wave + (uint32_t)i * (NT / 64) * 1024u);
     }
   }
 };
+
+// Operand reads of tiles in LDS.  For 16-bit types the per-lane byte offsets
+// are set once (the swizzle repeats every 16 rows, so other rows and stages
+// differ by constants); left to the compiler the swizzle was worked out again
+// for every chunk.  `at` is a tile's byte offset from the workgroup's LDS.
+template <typename T, int D>
+struct Operands {
+  typedef typename Mma<T>::V8 V8;
+  const char* lds;
+  int r, h;
+  __device__ __forceinline__ void init(const char* base, int r_, int h_) {
+    lds = base, r = r_, h = h_;
+  }
+  __device__ __forceinline__ V8 row(int at, int tile32, int ks) const {
+    return row_op<T, D>(lds + at, 32 * tile32 + r, ks, h);
+  }
+  __device__ __forceinline__ V8 col(int at, int d0, int mt, int kk) const {
+    return col_op<T, D>(lds + at, d0 + 32 * mt, 16 * kk);
+  }
+};
+template <typename T, int D>
+struct Operands16 {
+  typedef typename Mma<T>::V8 V8;
+  const char* lds;
+  uint32_t row_off[D / 16], col_off[D / 32][2];
+  __device__ __forceinline__ void init(const char* base, int r, int h) {
+    lds = base;
+    const int lane = threadIdx.x & 63, grp = lane >> 4, j = lane & 15, q = grp & 1, hh = grp >> 1;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      row_off[ks] = opaque((uint32_t)(swz<D>(r, 2 * ks + h) * 2));
+#pragma unroll
+    for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        col_off[mt][x] = opaque(
+            (uint32_t)(swz_elem<D>(8 * x + 4 * hh + (j >> 2), mt * 32 + 16 * q + 4 * (j & 3)) * 2));
+  }
+  __device__ __forceinline__ V8 row(int at, int tile32, int ks) const {
+    return as_vec8<T>(*reinterpret_cast<const u32x4*>(lds + row_off[ks] + at + tile32 * 64 * D));
+  }
+  // channels 32 mt .. of a tile; a constant first channel of 0 or 128
+  __device__ __forceinline__ V8 col(int at, int d0, int mt, int kk) const {
+    const char* p = lds + at + kk * 32 * D + (d0 >> 7) * 256;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + col_off[mt][0]));
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + col_off[mt][1]));
+    const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+    return as_vec8<T>(u32x4{a[0], a[1], b[0], b[1]});
+  }
+};
+template <int D>
+struct Operands<__bf16, D> : Operands16<__bf16, D> {};
+template <int D>
+struct Operands<_Float16, D> : Operands16<_Float16, D> {};
 
 struct Rows {          // a [batch, head, token] view
   const void* p;
@@ -242,9 +330,10 @@ struct KeyWalk {
     j = first;
     last = min(first + chunks, (n + KC - 1) / KC);
   }
-  // The next chunk with a valid key at or after j; false if there is none.
+  // The next chunk with a valid key among j, j + STEP, ..; false if there is none.
+  template <int STEP = 1>
   __device__ __forceinline__ bool find() {
-    for (; j < last; ++j) {
+    for (; j < last; j += STEP) {
       uint32_t any = 0;
 #pragma unroll
       for (int x = 0; x < KC / 32; ++x) {
@@ -257,6 +346,8 @@ struct KeyWalk {
     }
     return false;
   }
+  // a key below the valid prefix is masked: zeros must come from the copy
+  __device__ __forceinline__ bool holes() const { return words && !whole(); }
   __device__ __forceinline__ bool whole() const {
     uint32_t all = ~0u;
 #pragma unroll
@@ -265,9 +356,14 @@ struct KeyWalk {
   }
 };
 
-// valid bit of the key that accumulator element i of lane half h holds
-__device__ __forceinline__ bool acc_valid(uint32_t w, int i, int h) {
-  return (w >> (8 * (i >> 2) + 4 * h + (i & 3))) & 1u;
+// Whether the key that accumulator element i holds is valid: key 8 (i / 4) + i % 4
+// in the lanes of half 0, four on in half 1.  The two bits of the (uniform) word
+// become a lane mask on the scalar unit.
+__device__ __forceinline__ bool acc_valid(uint32_t w, int i) {
+  const int k = 8 * (i >> 2) + (i & 3);
+  const uint32_t lo = (uint32_t)((int32_t)(w << (31 - k)) >> 31);
+  const uint32_t hi = (uint32_t)((int32_t)(w << (27 - k)) >> 31);
+  return __builtin_amdgcn_inverse_ballot_w64((uint64_t)hi << 32 | lo);
 }
 
 // Eight consecutive channels of a row, as T.

@@ -13,7 +13,7 @@ namespace {
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// rows start 16-byte aligned, and a tile's rows lie within 31 bits of its first
+// rows start 16-byte aligned, and a tile's rows lie within 30 bits of its first
 bool rows_ok(const void* p, const int64_t* stride, int es) {
   int64_t low = 0;
   for (int x = 0; x < 3; ++x) {
@@ -30,7 +30,8 @@ int check(const vsa_cross* c) {
       c->heads % c->kv_heads || c->heads > 65535 || c->head_dim <= 0 || c->head_dim > 256 ||
       c->head_dim % 8 || c->sq <= 0 || c->skv <= 0 || c->skv > (1LL << 31) - 256 ||
       c->sq > ((1LL << 31) - 256) / (c->heads / c->kv_heads) || !(c->scale - c->scale == 0.f) ||
-      (c->key_mask && c->mask_stride < 0))
+      (c->key_mask && c->mask_stride < 0) || c->q_stride[2] < c->head_dim ||
+      c->k_stride[2] < c->head_dim || c->v_stride[2] < c->head_dim)
     return VSA_ERR_SHAPE;
   const int es = c->dtype == VSA_F32 ? 4 : 2;
   if (!rows_ok(c->q, c->q_stride, es) || !rows_ok(c->k, c->k_stride, es) ||
@@ -50,6 +51,7 @@ CrossArgs args(const vsa_cross* c) {
   a.sq = (int)c->sq, a.skv = (int)c->skv, a.dim = c->head_dim;
   a.scale = c->scale;
   a.c2 = c->scale * kLog2e;
+  if (a.c2 == 0.f) a.c2 = 1.17549435e-38f;   // masked scores stay -inf, all others 2^0
   return a;
 }
 

@@ -12,6 +12,7 @@
 // With splits the parts (O normalised, base-2 LSE) go to fp32 scratch and a
 // second kernel joins them by their LSE.
 #include <algorithm>
+#include <type_traits>
 
 #include "cross.h"
 
@@ -73,25 +74,27 @@ void cross_fwd_kernel(CrossArgs a) {
   const T* kbase = (const T*)a.k.p + b * a.k.b + kh * a.k.h;
   const T* vbase = (const T*)a.v.p + b * a.v.b + kh * a.v.h;
   TileCopy<T, D, KC, C::NT> kcopy, vcopy;
-  kcopy.init(a.k.s, a.dim);
-  vcopy.init(a.v.s, a.dim);
+  kcopy.init(a.k.s, a.dim, threadIdx.x);
+  vcopy.init(a.v.s, a.dim, threadIdx.x);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem));
-  const bool dim_full = a.dim == D;
+  Operands<T, D> ops;
+  ops.init(smem, r, h);
 
   const int chunks = (a.skv + KC - 1) / KC;
   const int per_split = (chunks + a.splits - 1) / a.splits;
   KeyWalk<KC> walk;
   walk.init(a, b, split * per_split, per_split);
-  auto copy = [&](int stage) {
-    const T* ks = kbase + (int64_t)walk.j * KC * a.k.s;
-    const T* vs = vbase + (int64_t)walk.j * KC * a.v.s;
+  auto copy = [&](int stage) __attribute__((always_inline)) {
+    const int left = walk.n - walk.j * KC;
+    const auto ks = kcopy.rows(kbase + (int64_t)walk.j * KC * a.k.s, left);
+    const auto vs = vcopy.rows(vbase + (int64_t)walk.j * KC * a.v.s, left);
     const uint32_t to = lds0 + stage * C::STAGE;
-    if (dim_full && walk.whole()) {
-      kcopy.whole(to, ks);
-      vcopy.whole(to + C::TILE, vs);
+    if (!walk.holes()) {
+      kcopy.copy(to, ks);
+      vcopy.copy(to + C::TILE, vs);
     } else {
-      kcopy.part(to, ks, walk.w);
-      vcopy.part(to + C::TILE, vs, walk.w);
+      kcopy.copy_valid(to, ks, walk.w);
+      vcopy.copy_valid(to + C::TILE, vs, walk.w);
     }
   };
 
@@ -105,8 +108,11 @@ void cross_fwd_kernel(CrossArgs a) {
   if (have) copy(0);
   dma_wait();
   __syncthreads();
-  int stage = 0;
-  while (have) {
+  // one chunk, of stage `stage` (a constant: every LDS address is a lane offset
+  // plus an immediate)
+  auto chunk = [&](auto stage_c) __attribute__((always_inline)) {
+    const int stage = stage_c;
+    const int Ks = stage * C::STAGE, Vs = Ks + C::TILE;
     uint32_t w[C::NSM];
 #pragma unroll
     for (int x = 0; x < C::NSM; ++x) w[x] = walk.w[x];
@@ -114,8 +120,6 @@ void cross_fwd_kernel(CrossArgs a) {
     ++walk.j;
     have = walk.find();
     if (have) copy(stage ^ 1);
-    const char* Ks = smem + stage * C::STAGE;
-    const char* Vs = Ks + C::TILE;
 
     f32x16 sacc[C::NSM];
 #pragma unroll
@@ -123,8 +127,7 @@ void cross_fwd_kernel(CrossArgs a) {
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
 #pragma unroll
-      for (int x = 0; x < C::NSM; ++x)
-        sacc[x] = M::mul(row_op<T, D>(Ks, 32 * x + r, ks, h), qf[ks], sacc[x]);
+      for (int x = 0; x < C::NSM; ++x) sacc[x] = M::mul(ops.row(Ks, x, ks), qf[ks], sacc[x]);
       step_fence<T, D>();
     }
     if (!whole) {
@@ -132,8 +135,7 @@ void cross_fwd_kernel(CrossArgs a) {
 #pragma unroll
       for (int x = 0; x < C::NSM; ++x)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (!acc_valid(w[x], i, h)) sacc[x][i] = -INFINITY;
+        for (int i = 0; i < 16; ++i) sacc[x][i] = acc_valid(w[x], i) ? sacc[x][i] : -INFINITY;
     }
     float m4[4] = {sacc[0][0], sacc[0][1], sacc[0][2], sacc[0][3]};
 #pragma unroll
@@ -156,14 +158,6 @@ void cross_fwd_kernel(CrossArgs a) {
     for (int x = 0; x < C::NSM; ++x)
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[x][i] = fast_exp2(fmaf(sacc[x][i], a.c2, negm));
-    if (!whole) {   // with c2 = 0 the masked scores' -inf is lost
-      keep_branch();
-#pragma unroll
-      for (int x = 0; x < C::NSM; ++x)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (!acc_valid(w[x], i, h)) p[x][i] = 0.f;
-    }
     float l4[4] = {p[0][0], p[0][1], p[0][2], p[0][3]};
 #pragma unroll
     for (int x = 4; x < 16 * C::NSM; ++x) l4[x & 3] += p[x >> 4][x & 15];
@@ -173,11 +167,19 @@ void cross_fwd_kernel(CrossArgs a) {
       const V8 bop = pack_op<T>(&p[kk >> 1][8 * (kk & 1)]);
 #pragma unroll
       for (int mt = 0; mt < D / 32; ++mt)
-        oacc[mt] = M::mul(col_op<T, D>(Vs, mt * 32, 16 * kk), bop, oacc[mt]), step_fence<T, D>();
+        oacc[mt] = M::mul(ops.col(Vs, 0, mt, kk), bop, oacc[mt]), step_fence<T, D>();
     }
     dma_wait();
     __syncthreads();
-    stage ^= 1;
+  };
+  if constexpr (kWide<T, D>) {   // two copies of the body do not fit its registers
+    for (int stage = 0; have; stage ^= 1) chunk(stage);
+  } else {
+    while (have) {
+      chunk(std::integral_constant<int, 0>{});
+      if (!have) break;
+      chunk(std::integral_constant<int, 1>{});
+    }
   }
 
   const float total = pair_sum32(lsum);
@@ -211,33 +213,284 @@ void cross_fwd_kernel(CrossArgs a) {
   if (store && h == 0 && a.lse) a.lse[stat] = any ? m + log2f(total) : -INFINITY;
 }
 
-// Joins the splits' parts: out = sum_s 2^(lse_s - L) O_s, L the row's LSE.  One
-// thread per eight channels of a row.
+// 32 NQ query rows of a (sample, key head) on its keys, for up to 64 of them: bound by reading K
+// and V, so the waves of a workgroup share the keys, not the rows.  Each walks
+// every NW-th chunk of 32 keys through a ring of its own in LDS (no barrier: a
+// wave waits for its own copies), and the parts meet in LDS at the end.
+// Splits over workgroups are for long keys alone.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
+struct CrossFewCfg {
+  static constexpr int TILE = 32 * D * (int)sizeof(T);
+  static constexpr int RING = 4 * TILE;                    // two chunks of K and V
+  static constexpr int NW = D == 64 ? 8 : D == 128 ? 4 : 2;
+  static constexpr int LDS = NW * RING;                    // 128 KiB
+  typedef TileCopy<T, D, 32, 64> Copy;
+};
+
+template <typename T, int D, int NQ>
+__global__ __launch_bounds__((CrossFewCfg<T, D>::NW * 64)) void cross_few_kernel(CrossArgs a) {
+  using C = CrossFewCfg<T, D>;
+  using M = Mma<T>;
+  typedef typename M::V8 V8;
+  constexpr int NW = C::NW, TT = NQ * (D / 32);
+  __shared__ __attribute__((aligned(16))) char smem[C::LDS];
+  __shared__ float stat_s[NW][NQ][2][64];
+  static_assert(NW * TT * 16 * 256 <= C::LDS, "the parts fit the rings");
+
+  const int own = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const int hk = own / a.per_head, row0 = own % a.per_head * 32 * NQ;
+  const int b = hk / a.kv_heads, kh = hk % a.kv_heads;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 31, h = lane >> 5;
   const int rows = a.group * a.sq;
-  const int64_t all = (int64_t)a.batch * a.kv_heads * rows;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t prow = id / (D / 8);
-  const int d = (int)(id % (D / 8)) * 8;
-  if (prow >= all) return;
-  float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_b[s * all + prow]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, acc[8] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float l = a.part_b[s * all + prow];
-    const float w = fast_exp2(l - base);
-    sum += w;
-    const float* p = a.part_a + (s * all + prow) * D + d;
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+  const char* ring = smem + wave * C::RING;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem)) + wave * C::RING;
+
+  const T* kbase = (const T*)a.k.p + b * a.k.b + kh * a.k.h;
+  const T* vbase = (const T*)a.v.p + b * a.v.b + kh * a.v.h;
+  typename C::Copy kcopy, vcopy;
+  kcopy.init(a.k.s, a.dim, lane);
+  vcopy.init(a.v.s, a.dim, lane);
+  const int chunks = (a.skv + 31) / 32;
+  const int per_split = (chunks + a.splits - 1) / a.splits;
+  KeyWalk<32> walk;
+  walk.init(a, b, split * per_split, per_split);
+  walk.j += wave;
+  uint32_t next_w = 0;
+  auto copy = [&](int stage) __attribute__((always_inline)) {
+    const int left = walk.n - walk.j * 32;
+    const auto ks = kcopy.rows(kbase + (int64_t)walk.j * 32 * a.k.s, left);
+    const auto vs = vcopy.rows(vbase + (int64_t)walk.j * 32 * a.v.s, left);
+    const uint32_t to = lds0 + stage * 2 * C::TILE;
+    if (!walk.holes()) {
+      kcopy.copy(to, ks);
+      vcopy.copy(to + C::TILE, vs);
+    } else {
+      kcopy.copy_valid(to, ks, walk.w);
+      vcopy.copy_valid(to + C::TILE, vs, walk.w);
+    }
+    next_w = walk.w[0];
+  };
+  uint32_t w = 0;
+  bool have = walk.template find<NW>();
+  if (have) {
+    copy(0);
+    w = next_w;
+    walk.j += NW;
+  }
+  bool ahead = have && walk.template find<NW>();
+  if (ahead) copy(1);
+  const bool any = have;
+
+  V8 qf[NQ][D / 16];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[e] = fmaf(w, x[e], acc[e]);
-      acc[4 + e] = fmaf(w, y[e], acc[4 + e]);
+  for (int t = 0; t < NQ; ++t) {
+    const int at = min(row0 + 32 * t + r, rows - 1);
+    const T* qrow = (const T*)a.q.p + b * a.q.b + (kh * a.group + at / a.sq) * a.q.h + at % a.sq * a.q.s;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const int d = 16 * ks + 8 * h;
+      V8 x = zero8<T>();
+      if (d < a.dim) x = ld8<T>(qrow + d);
+      u32x4 raw = __builtin_bit_cast(u32x4, x);
+      raw ^= a.qsign;   // a negative softmax scale
+      qf[t][ks] = as_vec8<T>(raw);
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  Operands<T, D> ops;
+  ops.init(ring, r, h);
+  float m[NQ], lsum[NQ];
+  f32x16 oacc[NQ][D / 32];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    m[t] = -INFINITY, lsum[t] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < D / 32; ++mt) oacc[t][mt] = f32x16{};
+  }
+  int stage = 0;
+  while (have) {
+    // this chunk has landed (the loads of the one ahead may be in flight)
+    if (ahead) wait_vmcnt<2 * C::Copy::N>();
+    else dma_wait();
+    asm volatile("" ::: "memory");   // no read of the stage moves before its wait
+    __builtin_amdgcn_sched_barrier(0);
+    const int Ks = stage * 2 * C::TILE, Vs = Ks + C::TILE;
+    f32x16 s[NQ];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) s[t] = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const V8 k = ops.row(Ks, 0, ks);
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) s[t] = M::mul(k, qf[t][ks], s[t]);
+    }
+    V8 bop[NQ][2];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      if (w != ~0u) {
+        keep_branch();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = acc_valid(w, i) ? s[t][i] : -INFINITY;
+      }
+      float m4[4] = {s[t][0], s[t][1], s[t][2], s[t][3]};
+#pragma unroll
+      for (int i = 4; i < 16; ++i) m4[i & 3] = vmax(m4[i & 3], s[t][i]);
+      const float smax = pair_max32(vmax(vmax(m4[0], m4[1]), vmax(m4[2], m4[3]))) * a.c2;
+      const bool grow = smax > m[t] + kSlack;
+      if (__any(grow)) {
+        const float mnew = grow ? smax : m[t];
+        const float alpha = m[t] == mnew ? 1.f : fast_exp2(m[t] - mnew);
+        lsum[t] *= alpha;
+#pragma unroll
+        for (int mt = 0; mt < D / 32; ++mt) oacc[t][mt] *= alpha;
+        m[t] = mnew;
+      }
+      const float negm = m[t] == -INFINITY ? 0.f : -m[t];
+      float p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = fast_exp2(fmaf(s[t][i], a.c2, negm));
+      float l4[4] = {p[0], p[1], p[2], p[3]};
+#pragma unroll
+      for (int i = 4; i < 16; ++i) l4[i & 3] += p[i];
+      lsum[t] += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+      bop[t][0] = pack_op<T>(p);
+      bop[t][1] = pack_op<T>(p + 8);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int mt = 0; mt < D / 32; ++mt) {
+        const V8 v = ops.col(Vs, 0, mt, kk);
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) oacc[t][mt] = M::mul(v, bop[t][kk], oacc[t][mt]);
+      }
+    // every read of this stage has returned (its product has been issued)
+    __builtin_amdgcn_sched_barrier(0);
+    have = ahead;
+    w = next_w;
+    if (have) {
+      walk.j += NW;
+      ahead = walk.template find<NW>();
+      if (ahead) copy(stage);
+    }
+    stage ^= 1;
+  }
+
+  // the waves' parts: their sums as registers of 64 lanes, their m and l
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    stat_s[wave][t][0][lane] = m[t];
+    stat_s[wave][t][1][lane] = pair_sum32(lsum[t]);
+  }
+  const bool some = __syncthreads_or(any);   // and every ring is done with
+  float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int t = 0; t < NQ; ++t)
+#pragma unroll
+    for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        part[((wave * TT + t * (D / 32) + mt) * 16 + i) * 64 + lane] = oacc[t][mt][i];
+  __syncthreads();
+  for (int x = wave; x < TT; x += NW) {
+    const int t = x / (D / 32), mt = x % (D / 32);
+    float top = -INFINITY, total = 0.f, weight[NW];
+#pragma unroll
+    for (int y = 0; y < NW; ++y) top = vmax(top, stat_s[y][t][0][lane]);
+#pragma unroll
+    for (int y = 0; y < NW; ++y) {
+      const float own = stat_s[y][t][0][lane];
+      // (a wave without a chunk has -inf and sums of 0; so has a row whose scores
+      // are all -inf, and then 0 / 0 below)
+      weight[y] = own == -INFINITY ? 0.f : fast_exp2(own - top);
+      total = fmaf(weight[y], stat_s[y][t][1][lane], total);
+    }
+    f32x16 o = f32x16{};
+#pragma unroll
+    for (int y = 0; y < NW; ++y)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        o[i] = fmaf(weight[y], part[((y * TT + x) * 16 + i) * 64 + lane], o[i]);
+    const float inv = some ? 1.0f / total : 0.f;
+    float w8[2][8];
+    swap_rows16(o, inv, w8);
+    const int row = row0 + 32 * t + r;
+    if (row >= rows) continue;
+    const int head = kh * a.group + row / a.sq, sq_i = row % a.sq;
+    const int64_t stat = ((int64_t)b * a.heads + head) * a.sq + sq_i;
+    const float lse = some ? top + log2f(total) : -INFINITY;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const int d = mt * 32 + 16 * z + 8 * h;
+      if (a.splits > 1) {
+        st8<float>(a.part_a + (((int64_t)split * a.batch * a.kv_heads + hk) * rows + row) * D + d, w8[z]);
+      } else if (d < a.dim) {
+        st8_out<T>((T*)a.out + b * a.out_s[0] + head * a.out_s[1] + sq_i * a.out_s[2] + d,
+                   a.lo ? (T*)a.lo + stat * a.dim + d : nullptr, w8[z]);
+      }
+    }
+    if (h == 0 && mt == 0) {
+      if (a.splits > 1) a.part_b[((int64_t)split * a.batch * a.kv_heads + hk) * rows + row] = lse;
+      else if (a.lse) a.lse[stat] = lse;
+    }
+  }
+}
+
+// Joins the splits' parts: out = sum_s 2^(lse_s - L) O_s / sum_s 2^(lse_s - L).  A
+// row has D / 8 threads of eight channels, times `lanes` that take every
+// lanes-th split each and meet in LDS (one thread a row's piece walked a hundred
+// splits alone: 52 us for 64 queries on 40960 keys, as long as the attention).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a, int lanes) {
+  constexpr int W = D / 8;
+  __shared__ float acc_s[256][9];
+  __shared__ float top_s[256];
+  const int rows = a.group * a.sq;
+  const int64_t all = (int64_t)a.batch * a.kv_heads * rows;
+  const int piece = threadIdx.x % W, lane = threadIdx.x / W % lanes;
+  const int64_t prow = (int64_t)blockIdx.x * (256 / W / lanes) + threadIdx.x / W / lanes;
+  const int d = piece * 8;
+  float top = -INFINITY, sum = 0.f, acc[8] = {};
+  if (prow < all) {
+    for (int s = lane; s < a.splits; s += lanes) {
+      const float* p = a.part_a + (s * all + prow) * D + d;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+      const float l = a.part_b[s * all + prow];
+      if (l == -INFINITY) continue;
+      const float next = fmaxf(top, l), scale = fast_exp2(top - next), w = fast_exp2(l - next);
+      top = next;
+      sum = fmaf(sum, scale, w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[e] = fmaf(acc[e], scale, w * x[e]);
+        acc[4 + e] = fmaf(acc[4 + e], scale, w * y[e]);
+      }
+    }
+  }
+  if (lanes > 1) {
+    top_s[threadIdx.x] = top;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc_s[threadIdx.x][e] = acc[e];
+    acc_s[threadIdx.x][8] = sum;
+    __syncthreads();
+    if (lane) return;
+    float t = top;
+    for (int x = 1; x < lanes; ++x) t = fmaxf(t, top_s[threadIdx.x + x * W]);
+    const float own = top == -INFINITY ? 0.f : fast_exp2(top - t);
+    sum *= own;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= own;
+    for (int x = 1; x < lanes; ++x) {
+      const int at = threadIdx.x + x * W;
+      const float w = top_s[at] == -INFINITY ? 0.f : fast_exp2(top_s[at] - t);
+      sum = fmaf(w, acc_s[at][8], sum);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, acc_s[at][e], acc[e]);
+    }
+    top = t;
+  }
+  if (prow >= all) return;
+  const float inv = top == -INFINITY ? 0.f : 1.0f / sum;
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] *= inv;
   const int hk = (int)(prow / rows), i = (int)(prow % rows);
@@ -246,7 +499,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
   if (d < a.dim)
     st8_out<T>((T*)a.out + b * a.out_s[0] + head * a.out_s[1] + (i % a.sq) * a.out_s[2] + d,
                a.lo ? (T*)a.lo + stat * a.dim + d : nullptr, acc);
-  if (d == 0 && a.lse) a.lse[stat] = top == -INFINITY ? top : base + log2f(sum);
+  if (d == 0 && a.lse) a.lse[stat] = top == -INFINITY ? top : top + log2f(sum);
 }
 
 // 32 keys of a sample to a word: its key_mask and its kv_lens.
@@ -266,7 +519,8 @@ __global__ __launch_bounds__(256) void cross_words_kernel(const uint8_t* __restr
 namespace {
 
 struct Plan {
-  int nw, kd, splits, per_head;
+  int kd, nw, nq;      // nq: 32-row tiles of the few-row kernel, 0 for the other
+  int splits, per_head;
   int64_t tiles;
 };
 
@@ -275,12 +529,27 @@ int fwd_kc(const vsa_cross* c, int kd, int nw) {
 }
 
 Plan fwd_plan(const vsa_cross* c) {
-  Plan p;
-  const int64_t rows = c->heads / c->kv_heads * c->sq;
+  Plan p = {};
+  const int64_t rows = c->heads / c->kv_heads * c->sq, heads = (int64_t)c->batch * c->kv_heads;
   p.kd = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
-  p.nw = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  if (c->dtype != VSA_F32 && rows <= 64) {
+    p.nq = rows <= 32 || p.kd == 256 ? 1 : 2;   // (two at head dim 256 spill)
+    p.nw = p.kd == 64 ? 8 : p.kd == 128 ? 4 : 2;
+    p.per_head = (int)((rows + 32 * p.nq - 1) / (32 * p.nq));
+    p.tiles = heads * p.per_head;
+    // a workgroup a CU; splits only where a wave has more than eight chunks
+    const int64_t chunks = (c->skv + 31) / 32;
+    int64_t splits = std::max<int64_t>(1, cu_count() / p.tiles);
+    splits = std::max<int64_t>(1, std::min(splits, chunks / (8 * p.nw)));
+    const int64_t per = (chunks + splits - 1) / splits;
+    p.splits = (int)((chunks + per - 1) / per);
+    return p;
+  }
+  // (two waves at least for fp32 at head dim 256: one has too many pieces to copy)
+  const bool wide = c->dtype == VSA_F32 && p.kd == 256;
+  p.nw = rows <= 32 && !wide ? 1 : rows <= 64 ? 2 : 4;
   p.per_head = (int)((rows + 32 * p.nw - 1) / (32 * p.nw));
-  p.tiles = (int64_t)c->batch * c->kv_heads * p.per_head;
+  p.tiles = heads * p.per_head;
   // workgroups that the chip holds at once, by their LDS
   const int kc = fwd_kc(c, p.kd, p.nw);
   const int lds = 4 * kc * p.kd * (c->dtype == VSA_F32 ? 4 : 2);
@@ -309,18 +578,36 @@ int cross_words(const vsa_cross* c, uint32_t* words, int nwords, hipStream_t s) 
   return vsa_check_launch();
 }
 
-template <typename T, int D, int NW>
-static int launch_fwd(const CrossArgs& a, hipStream_t s) {
-  using C = CrossFwdCfg<T, D, NW>;
-  const int grid = (a.tiles * a.splits + 7) / 8 * 8;
-  static_assert(2 * C::STAGE <= 160 * 1024, "");
-  hipLaunchKernelGGL((cross_fwd_kernel<T, D, NW>), dim3((unsigned)grid), dim3(C::NT), 0, s, a);
+template <typename T, int D>
+static int launch_fwd(const Plan& p, const CrossArgs& a, hipStream_t s) {
+  const unsigned grid = (unsigned)((p.tiles * p.splits + 7) / 8 * 8);
+  if constexpr (sizeof(T) == 2) {
+    const dim3 few((unsigned)(p.tiles * p.splits)), nt(CrossFewCfg<T, D>::NW * 64);
+    if (p.nq == 1) hipLaunchKernelGGL((cross_few_kernel<T, D, 1>), few, nt, 0, s, a);
+    else if (p.nq == 0) hipLaunchKernelGGL((cross_fwd_kernel<T, D, 4>), dim3(grid), dim3(256), 0, s, a);
+    else if constexpr (D < 256) hipLaunchKernelGGL((cross_few_kernel<T, D, 2>), few, nt, 0, s, a);
+  } else {
+    if (p.nw == 4) hipLaunchKernelGGL((cross_fwd_kernel<T, D, 4>), dim3(grid), dim3(256), 0, s, a);
+    else if (D == 256 || p.nw == 2)
+      hipLaunchKernelGGL((cross_fwd_kernel<T, D, 2>), dim3(grid), dim3(128), 0, s, a);
+    else if constexpr (D < 256)
+      hipLaunchKernelGGL((cross_fwd_kernel<T, D, 1>), dim3(grid), dim3(64), 0, s, a);
+  }
   const int rc = vsa_check_launch();
-  if (rc || a.splits == 1) return rc;
-  const int64_t n = (int64_t)a.batch * a.heads * a.sq * (D / 8);
-  hipLaunchKernelGGL((cross_join_kernel<T, D>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,
-                     a);
+  if (rc || p.splits == 1) return rc;
+  int lanes = 1;   // a power of two up to the threads that a row can have
+  while (lanes < a.splits && lanes < 256 / (D / 8)) lanes *= 2;
+  const int64_t n = (int64_t)a.batch * a.heads * a.sq, per = 256 / (D / 8) / lanes;
+  hipLaunchKernelGGL((cross_join_kernel<T, D>), dim3((unsigned)((n + per - 1) / per)), dim3(256), 0,
+                     s, a, lanes);
   return vsa_check_launch();
+}
+
+template <typename T>
+static int fwd_of(const Plan& p, const CrossArgs& a, hipStream_t s) {
+  if (p.kd == 64) return launch_fwd<T, 64>(p, a, s);
+  if (p.kd == 128) return launch_fwd<T, 128>(p, a, s);
+  return launch_fwd<T, 256>(p, a, s);
 }
 
 int cross_fwd(const vsa_cross* c, CrossArgs a, char* scratch, hipStream_t s) {
@@ -333,18 +620,7 @@ int cross_fwd(const vsa_cross* c, CrossArgs a, char* scratch, hipStream_t s) {
     a.part_a = (float*)scratch;
     a.part_b = a.part_a + (int64_t)c->batch * c->heads * c->sq * p.splits * p.kd;
   }
-#define VSA_CROSS_NW(T, D)                             \
-  do {                                                 \
-    if (p.nw == 1) return launch_fwd<T, D, 1>(a, s);   \
-    if (p.nw == 2) return launch_fwd<T, D, 2>(a, s);   \
-    return launch_fwd<T, D, 4>(a, s);                  \
-  } while (0)
-  VSA_DISPATCH_ALL(c->dtype, T, {
-    if (p.kd == 64) VSA_CROSS_NW(T, 64);
-    if (p.kd == 128) VSA_CROSS_NW(T, 128);
-    VSA_CROSS_NW(T, 256);
-  });
-#undef VSA_CROSS_NW
+  VSA_DISPATCH_ALL(c->dtype, T, return fwd_of<T>(p, a, s));
 }
 
 }  // namespace vsa

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from typing import Optional
 
@@ -87,29 +88,13 @@ class VsaOp(ctypes.Structure):
                 + [("scale", _F)])
 
 
-class VsaRotaryAxis(ctypes.Structure):
-    """``struct vsa_rotary_axis`` of the header."""
-    _fields_ = ([(n, _I32) for n in ("positions", "channels", "method", "reserved")]
-                + [(n, ctypes.c_double) for n in ("start", "theta", "factor", "original")])
-
-
-class VsaRotaryOp(ctypes.Structure):
-    """``struct vsa_rotary_op`` of the header."""
-    _fields_ = ([(n, _P) for n in ("q", "k", "q_out", "k_out", "cos", "sin", "positions")]
-                + [(n, _I64 * 3) for n in ("q_stride", "k_stride", "q_out_stride",
-                                           "k_out_stride")]
-                + [(n, _I64) for n in ("positions_stride", "batch", "tokens", "rows")]
-                + [(n, _I32) for n in ("q_heads", "k_heads", "head_dim", "channels",
-                                       "interleaved", "inverse", "positions64", "dtype")])
-
-
-class VsaCross(ctypes.Structure):
-    """``struct vsa_cross`` of the header."""
-    _fields_ = ([(n, _P) for n in ("q", "k", "v", "kv_lens", "key_mask")]
-                + [(n, _I64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
-                + [(n, _I64) for n in ("mask_stride", "sq", "skv")]
-                + [(n, _I32) for n in ("batch", "heads", "kv_heads", "head_dim", "dtype")]
-                + [("scale", _F)])
+# The other operators' structs, packed as bytes (a ctypes structure of this many
+# fields costs a small call more than its kernel does): struct vsa_rotary_axis[3],
+# vsa_rotary_op and vsa_cross of the header, fields in order.
+ROTARY_AXES = struct.Struct("4i4d" * 3)
+ROTARY_OP = struct.Struct("7P16q8i")
+CROSS = struct.Struct("5P12q5if")
+STRIDES = struct.Struct("3q")
 
 
 _lock = threading.Lock()

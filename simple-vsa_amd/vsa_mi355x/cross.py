@@ -34,51 +34,62 @@ def _rows16(x: Tensor) -> Tensor:
     other, every row 16-byte aligned, a tile's rows within reach of a 32-bit
     offset), else a dense copy."""
     es = x.element_size()
-    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0:
-        st = [n for n, size in zip(x.stride()[:3], x.shape[:3]) if size > 1]
-        if all(n * es % 16 == 0 for n in st) and \
-                (x.shape[2] == 1 or x.stride(2) <= (1 << 30) // (64 * es)):
+    if x.stride(3) == 1 and x.data_ptr() % 16 == 0:
+        b, h, s = _strides(x)
+        if (b | h | s) * es % 16 == 0 and x.shape[3] <= s <= (1 << 30) // (64 * es):
             return x
-    return x.clone() if x.is_contiguous() else x.contiguous()
+    return x.clone(memory_format=torch.contiguous_format)
 
 
-def _struct(q, k, v, lens, mask, scale) -> _lib.VsaCross:
-    return _lib.VsaCross(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lens), _ptr(mask), strides(q), strides(k),
-        strides(v), 0 if mask is None else mask.stride(0), q.shape[2], k.shape[2], q.shape[0],
-        q.shape[1], k.shape[1], q.shape[3], _lib.dtype_code(q.dtype), scale)
+def _strides(x: Tensor):
+    """Strides for the C ABI; those of a row where there is one token."""
+    b, h, s = strides(x)
+    return b, h, s if x.shape[2] > 1 else x.shape[3]
+
+
+def _pack(q, k, v, lens, mask, scale) -> bytes:
+    b, h, sq, d = q.shape
+    return _lib.CROSS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if lens is None else lens.data_ptr(),
+        0 if mask is None else mask.data_ptr(), *_strides(q), *_strides(k), *_strides(v),
+        0 if mask is None else mask.stride(0), sq, k.shape[2], b, h, k.shape[1], d,
+        _lib.DTYPE_CODES[q.dtype], scale)
+
+
+def _three(x: Tensor) -> bytes:
+    return _lib.STRIDES.pack(*_strides(x))
 
 
 @functools.lru_cache(maxsize=256)
 def _sizes(b, h, hk, sq, skv, d, masked, dtype):
     """Bytes of (forward scratch, backward scratch)."""
-    some, zero = 256, (ctypes.c_int64 * 3)()   # any aligned pointer: only its presence is read
-    c = _lib.VsaCross(some, some, some, None, some if masked else None, zero, zero, zero, 0, sq,
-                      skv, b, h, hk, d, dtype, 1.0)
+    # a pointer's presence is all that is read
+    c = _lib.CROSS.pack(256, 256, 256, 0, 256 if masked else 0, *(0, 0, 256) * 3, 0, sq, skv, b, h,
+                        hk, d, dtype, 1.0)
     n = (ctypes.c_int64 * 2)()
     at = ctypes.addressof(n)
-    _lib.call("vsa_cross_sizes", ctypes.addressof(c), at, at + 8)
+    _lib.call("vsa_cross_sizes", c, at, at + 8)
     return tuple(n)
 
 
-def _scratch(c: _lib.VsaCross, masked: bool, which: int, device) -> Optional[Tensor]:
-    return _workspace(_sizes(c.batch, c.heads, c.kv_heads, c.sq, c.skv, c.head_dim, masked,
-                             c.dtype)[which], device)
+def _scratch(q, k, masked: bool, which: int) -> Optional[Tensor]:
+    b, h, sq, d = q.shape
+    return _workspace(_sizes(b, h, k.shape[1], sq, k.shape[2], d, masked,
+                             _lib.DTYPE_CODES[q.dtype])[which], q.device)
 
 
 def _forward(q, k, v, lens, mask, scale, keep):
     """(out, lo, lse); the last two only where the backward needs them (``keep``)."""
     dev = q.device
     with on_device(dev):
-        c = _struct(q, k, v, lens, mask, scale)
         out = empty_in_order(q)
         lo = lse = None
         if keep:
             lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
             if q.dtype != torch.float32:
                 lo = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        scratch, st = _scratch(c, mask is not None, 0, dev), strides(out)
-        _lib.call("vsa_cross_fwd", ctypes.addressof(c), out.data_ptr(), ctypes.addressof(st),
+        scratch = _scratch(q, k, mask is not None, 0)
+        _lib.call("vsa_cross_fwd", _pack(q, k, v, lens, mask, scale), out.data_ptr(), _three(out),
                   _ptr(lo), _ptr(lse), _ptr(scratch),
                   torch._C._cuda_getCurrentRawStream(dev.index))
     return out, lo, lse
@@ -90,14 +101,11 @@ def _backward(q, k, v, lens, mask, scale, out, lo, lse, dout):
         # (the saved ones too: a saved-tensor hook may give back other addresses)
         q, k, v, out, dout = (_rows16(x) for x in (q, k, v, out, dout))
         lo = lo if lo is None else _rows16(lo.contiguous())
-        c = _struct(q, k, v, lens, mask, scale)
         dq, dk, dv = (empty_in_order(x) for x in (q, k, v))
-        scratch = _scratch(c, mask is not None, 1, dev)
-        s = [strides(x) for x in (out, dout, dq, dk, dv)]
-        at = [ctypes.addressof(x) for x in s]
-        _lib.call("vsa_cross_bwd", ctypes.addressof(c), out.data_ptr(), at[0], _ptr(lo),
-                  dout.data_ptr(), at[1], lse.data_ptr(), dq.data_ptr(), at[2], dk.data_ptr(), at[3],
-                  dv.data_ptr(), at[4], _ptr(scratch),
+        scratch = _scratch(q, k, mask is not None, 1)
+        _lib.call("vsa_cross_bwd", _pack(q, k, v, lens, mask, scale), out.data_ptr(), _three(out),
+                  _ptr(lo), dout.data_ptr(), _three(dout), lse.data_ptr(), dq.data_ptr(),
+                  _three(dq), dk.data_ptr(), _three(dk), dv.data_ptr(), _three(dv), _ptr(scratch),
                   torch._C._cuda_getCurrentRawStream(dev.index))
     return dq, dk, dv
 
@@ -151,10 +159,11 @@ def _check(q, k, v, kv_lens, key_mask, sm_scale) -> None:
             (h and sq > MAX_TOKENS // (h // k.shape[1])):
         raise ValueError("the MI355X kernels support at most 65535 samples and heads, and fewer "
                          "than 2^31 query rows of a key head and keys")
-    tensors = [x for x in (q, k, v, kv_lens, key_mask) if x is not None]
-    if not all(x.is_cuda for x in tensors):
+    if not q.is_cuda:
         raise ValueError("the MI355X implementation requires GPU tensors")
-    if any(x.device != q.device for x in tensors):
+    dev = q.device
+    if not (k.device == dev and v.device == dev and (kv_lens is None or kv_lens.device == dev)
+            and (key_mask is None or key_mask.device == dev)):
         raise ValueError("q, k, v, kv_lens and key_mask must be on the same GPU device")
 
 

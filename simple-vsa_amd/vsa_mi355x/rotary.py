@@ -10,7 +10,6 @@ Nothing here runs on the CPU: a CPU tensor or a missing kernel library raises.
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Tuple, Union
 
@@ -84,13 +83,13 @@ def build_rotary_table(dit_seq_shape: Tuple[int, int, int], axis_channels: Tuple
         raise ValueError("the MI355X implementation requires a GPU device")
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    axes = (_lib.VsaRotaryAxis * 3)(*(
-        _lib.VsaRotaryAxis(shape[i], channels[i], ROTARY_METHODS.index(method), 0, start[i], theta,
-                           factor[i], original[i]) for i in range(3)))
+    kind = ROTARY_METHODS.index(method)
+    axes = _lib.ROTARY_AXES.pack(*(x for i in range(3) for x in (
+        shape[i], channels[i], kind, 0, start[i], theta, factor[i], original[i])))
     cos = torch.empty((math.prod(shape), sum(channels) // 2), dtype=torch.float32, device=device)
     sin = torch.empty_like(cos)
     with on_device(device):
-        _lib.call("vsa_rotary_table", ctypes.addressof(axes), cos.data_ptr(), sin.data_ptr(),
+        _lib.call("vsa_rotary_table", axes, cos.data_ptr(), sin.data_ptr(),
                   torch._C._cuda_getCurrentRawStream(device.index))
     return cos, sin
 
@@ -113,29 +112,34 @@ def empty_in_order(x: Tensor, shape=None) -> Tensor:
     return torch.empty((b, h, s, d), dtype=x.dtype, device=x.device)
 
 
-def strides(x: Tensor):
+def strides(x: Tensor) -> Tuple[int, int, int]:
     """Strides of batch, head and token for the C ABI; 0 for a dimension of one."""
-    return (ctypes.c_int64 * 3)(*(n if size > 1 else 0
-                                  for n, size in zip(x.stride(), x.shape[:3])))
+    (b, h, s, _), (sb, sh, ss, _) = x.shape, x.stride()
+    return (sb if b > 1 else 0, sh if h > 1 else 0, ss if s > 1 else 0)
 
 
 def _rotate(q, k, cos, sin, positions, interleaved, inverse):
     """One launch: (q turned, k turned); k may be None."""
-    q, k = (x if x is None or x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
-            for x in (q, k))
-    q_out, k_out = empty_in_order(q), None if k is None else empty_in_order(k)
+    q_out = empty_in_order(q)
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    k_out = None
+    kk, ko, hk = q, q_out, 0
+    if k is not None:
+        k_out = ko = empty_in_order(k)
+        kk, hk = k if k.stride(3) == 1 else k.contiguous(), k.shape[1]
     b, h, s, d = q.shape
-    kk, ko = (q, q_out) if k is None else (k, k_out)
-    op = _lib.VsaRotaryOp(
+    rows, pairs = cos.shape
+    op = _lib.ROTARY_OP.pack(
         q.data_ptr(), kk.data_ptr(), q_out.data_ptr(), ko.data_ptr(), cos.data_ptr(),
-        sin.data_ptr(), None if positions is None else positions.data_ptr(), strides(q),
-        strides(kk), strides(q_out), strides(ko),
-        0 if positions is None or positions.dim() == 1 else s, b, s, cos.shape[0], h,
-        0 if k is None else k.shape[1], d, 2 * cos.shape[1], interleaved, inverse,
-        positions is not None and positions.dtype is torch.int64, _lib.dtype_code(q.dtype))
-    with on_device(q.device):
-        _lib.call("vsa_rotary", ctypes.addressof(op),
-                  torch._C._cuda_getCurrentRawStream(q.device.index))
+        sin.data_ptr(), 0 if positions is None else positions.data_ptr(), *strides(q),
+        *strides(kk), *strides(q_out), *strides(ko),
+        0 if positions is None or positions.dim() == 1 else s, b, s, rows, h, hk, d, 2 * pairs,
+        interleaved, inverse, positions is not None and positions.dtype is torch.int64,
+        _lib.DTYPE_CODES[q.dtype])
+    dev = q.device
+    with on_device(dev):
+        _lib.call("vsa_rotary", op, torch._C._cuda_getCurrentRawStream(dev.index))
     return q_out, k_out
 
 
@@ -192,10 +196,11 @@ def _check_rotary(q, k, cos, sin, positions) -> None:
             raise ValueError("positions must have shape [seq_len] or [batch, seq_len]")
         if cos.shape[0] == 0:
             raise ValueError("the table has no positions")
-    tensors = [x for x in (q, k, cos, sin, positions) if x is not None]
-    if not all(x.is_cuda for x in tensors):
+    if not q.is_cuda:
         raise ValueError("the MI355X implementation requires GPU tensors")
-    if any(x.device != q.device for x in tensors):
+    dev = q.device
+    if not (cos.device == dev and sin.device == dev and (k is None or k.device == dev)
+            and (positions is None or positions.device == dev)):
         raise ValueError("q, k, the table and the positions must be on the same GPU device")
 
 

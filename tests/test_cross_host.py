@@ -41,6 +41,22 @@ def test_refusals(kw, text):
         mi355x_cross_attention(**_args(**kw))
 
 
+_P, _I64, _I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+
+
+class Cross(ctypes.Structure):
+    """``struct vsa_cross`` of the header."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "kv_lens", "key_mask")]
+                + [(n, _I64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [(n, _I64) for n in ("mask_stride", "sq", "skv")]
+                + [(n, _I32) for n in ("batch", "heads", "kv_heads", "head_dim", "dtype")]
+                + [("scale", ctypes.c_float)])
+
+
+def test_packed_struct_has_the_headers_size():
+    assert _lib.CROSS.size == ctypes.sizeof(Cross)
+
+
 def test_entry_points_refuse_without_a_launch():
     lib = _lib.load()
     buf = torch.zeros(256)
@@ -51,7 +67,7 @@ def test_entry_points_refuse_without_a_launch():
     s3 = ctypes.addressof(st)
 
     def struct(**kw):
-        c = _lib.VsaCross()
+        c = Cross()
         c.q = c.k = c.v = p
         c.q_stride[:] = c.k_stride[:] = c.v_stride[:] = [64, 64, 64]
         c.sq, c.skv, c.batch, c.heads, c.kv_heads, c.head_dim = 4, 6, 2, 4, 2, 64
@@ -71,9 +87,10 @@ def test_entry_points_refuse_without_a_launch():
     assert sizes(q=None) == -1 and sizes(dtype=9) == -3
     for kw in (dict(batch=0), dict(heads=3), dict(kv_heads=0), dict(head_dim=60),
                dict(head_dim=264), dict(sq=0), dict(skv=0), dict(skv=1 << 31), dict(sq=1 << 31),
-               dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=65536)):
+               dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=65536),
+               dict(v_stride=[64, 64, 32])):
         assert sizes(**kw) == -2, kw
-    assert sizes(k=p + 8) == -7 and sizes(v_stride=[64, 64, 4]) == -7
+    assert sizes(k=p + 8) == -7 and sizes(v_stride=[64, 4, 64]) == -7
     assert sizes(q_stride=[-64, 64, 64]) == -7 and sizes(k_stride=[64, 64, 1 << 30]) == -7
     assert sizes(kv_lens=p + 2) == -7
     c = struct()
@@ -100,8 +117,9 @@ def test_workspaces_are_bounded():
     at = ctypes.addressof(n)
     for b, h, sq, skv, d in ((1, 12, 64, 40960, 128), (8, 12, 1, 512, 128),
                              (1, 40, 40960, 512, 128), (1, 1, 1, 1 << 20, 64)):
-        c = _lib.VsaCross()
+        c = Cross()
         c.q = c.k = c.v = 256
+        c.q_stride[:] = c.k_stride[:] = c.v_stride[:] = [256, 256, 256]
         c.sq, c.skv, c.batch, c.heads, c.kv_heads, c.head_dim, c.scale = sq, skv, b, h, h, d, 1.0
         assert lib.vsa_cross_sizes(ctypes.addressof(c), at, at + 8) == 0
         assert n[0] <= 1 << 28 and n[1] <= 1 << 30, (n[0], n[1])

@@ -65,12 +65,36 @@ def test_tiled_op_checks_its_table():
         mi355x_vsa_tiled(q, q, q, (2, 2, 2), 1, rotary=(torch.zeros(7, 32), torch.zeros(7, 32)))
 
 
+_P, _I64, _I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+
+
+class Axis(ctypes.Structure):
+    """``struct vsa_rotary_axis`` of the header."""
+    _fields_ = ([(n, _I32) for n in ("positions", "channels", "method", "reserved")]
+                + [(n, ctypes.c_double) for n in ("start", "theta", "factor", "original")])
+
+
+class Op(ctypes.Structure):
+    """``struct vsa_rotary_op`` of the header."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "q_out", "k_out", "cos", "sin", "positions")]
+                + [(n, _I64 * 3) for n in ("q_stride", "k_stride", "q_out_stride",
+                                           "k_out_stride")]
+                + [(n, _I64) for n in ("positions_stride", "batch", "tokens", "rows")]
+                + [(n, _I32) for n in ("q_heads", "k_heads", "head_dim", "channels",
+                                       "interleaved", "inverse", "positions64", "dtype")])
+
+
+def test_packed_structs_have_the_headers_size():
+    assert _lib.ROTARY_AXES.size == ctypes.sizeof(Axis * 3)
+    assert _lib.ROTARY_OP.size == ctypes.sizeof(Op)
+
+
 def test_entry_points_refuse_without_a_launch():
     lib = _lib.load()
     buf = torch.zeros(64)
     p = (buf.data_ptr() + 15) // 16 * 16
-    axes = (_lib.VsaRotaryAxis * 3)(*(_lib.VsaRotaryAxis(2, 4, 0, 0, 0.0, 1e4, 1.0, 0.0)
-                                      for _ in range(3)))
+    axes = (Axis * 3)(*(Axis(2, 4, 0, 0, 0.0, 1e4, 1.0, 0.0)
+                    for _ in range(3)))
     at = ctypes.addressof(axes)
     assert lib.vsa_rotary_table(None, p, p, None) == -1
     assert lib.vsa_rotary_table(at, p + 2, p, None) == -7
@@ -84,7 +108,7 @@ def test_entry_points_refuse_without_a_launch():
     assert lib.vsa_rotary_table(at, p, p, None) == -2    # yarn without the trained length
 
     def op(**kw):
-        o = _lib.VsaRotaryOp()
+        o = Op()
         for n in ("q", "k", "q_out", "k_out", "cos", "sin"):
             setattr(o, n, p)
         o.batch = o.tokens = o.rows = o.q_heads = o.k_heads = 1

@@ -517,8 +517,8 @@ int vsa_rotary(const vsa_rotary_op* op, void* stream);
  * left over, which a backward with it takes its row sums of dout * out from
  * (without it dq loses up to two bits; unused in fp32).  dk and dv are written for every
  * key (zeros where it is not valid) and summed over the heads that share a key
- * head, in a fixed order.  Scratch sizes come from vsa_cross_sizes (256-byte
- * aligned; 0: NULL will do).
+ * head, in a fixed order.  Scratch sizes come from vsa_cross_sizes, from
+ * the sizes and from which pointers are NULL (256-byte aligned; 0: NULL will do).
  */
 typedef struct vsa_cross {
   const void *q, *k, *v;

@@ -78,6 +78,14 @@ __device__ __forceinline__ void step_fence() {
   if constexpr (kWide<T, D>) __builtin_amdgcn_sched_barrier(0);
 }
 
+// Whether the channels from d on take part in a product.  fp32 products of 16
+// channels take 512 cycles, a scalar branch pays for leaving out those past the
+// head dim (80 of 128: TIMES2); at 16 bits, 32 cycles, it would not.
+template <typename T>
+__device__ __forceinline__ bool in_dim(int d, int dim) {
+  return sizeof(T) == 2 || d < dim;
+}
+
 // LDS tile of rows of D elements, 16-byte chunks swizzled by the row: 16-bit
 // types as in vsa_device.h, fp32 rows (at least 256 bytes: one pass over the 64
 // banks) by the row's low four bits.
@@ -306,9 +314,19 @@ struct CrossArgs {
   int sq, skv, heads, kv_heads, group, dim;
   int batch, splits, tiles;    // tiles of a split
   int per_head;                // tiles of a (batch, key head)
+  int spread;                  // order of the tiles: see tile_of
   float c2, scale;
   uint32_t qsign;
 };
+
+// The tile of a workgroup.  An XCD takes a contiguous range (xcd_tile), so that
+// the K and V of a head stay in its L2.  Where samples may differ in their keys
+// and one head's K and V are small, tiles go round the XCDs instead: by ranges
+// the XCDs of the samples with few keys end early (2 samples of 10 heads, 3001
+// queries in fp32 on 333 keys and on none: TIMES).
+__device__ __forceinline__ int tile_of(const CrossArgs& a) {
+  return a.spread ? (int)blockIdx.x : xcd_tile(blockIdx.x, a.tiles * a.splits);
+}
 
 typedef const __attribute__((address_space(4))) uint32_t* const_words;
 

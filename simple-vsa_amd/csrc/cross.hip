@@ -49,6 +49,8 @@ CrossArgs args(const vsa_cross* c) {
   a.batch = c->batch, a.heads = c->heads, a.kv_heads = c->kv_heads;
   a.group = c->heads / c->kv_heads;
   a.sq = (int)c->sq, a.skv = (int)c->skv, a.dim = c->head_dim;
+  a.spread = c->batch > 1 && (c->kv_lens || c->key_mask) &&
+             2 * c->skv * c->head_dim * (c->dtype == VSA_F32 ? 4 : 2) <= 1 << 20;
   a.scale = c->scale;
   a.c2 = c->scale * kLog2e;
   if (a.c2 == 0.f) a.c2 = 1.17549435e-38f;   // masked scores stay -inf, all others 2^0

@@ -38,14 +38,14 @@ void cross_dq_kernel(CrossArgs a) {
   constexpr int KC = C::KC;
   __shared__ __attribute__((aligned(16))) char smem[2 * C::STAGE];
 
-  const int tile = xcd_tile(blockIdx.x, a.tiles * a.splits);
+  const int tile = tile_of(a);
   if (tile >= a.tiles * a.splits) return;
   const int split = tile % a.splits, own = tile / a.splits;
-  const int hk = own / a.per_head;
+  const int hk = own / a.per_head;                  // batch * kv_heads + key head
   const int b = hk / a.kv_heads, kh = hk % a.kv_heads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 31, h = lane >> 5;
-  const int row = (own % a.per_head) * (32 * NW) + wave * 32 + r;
+  const int row = own % a.per_head * (32 * NW) + wave * 32 + r;
   const int rows = a.group * a.sq;
   const int at = min(row, rows - 1);
   const int head = kh * a.group + at / a.sq, sq_i = at % a.sq;
@@ -151,6 +151,7 @@ void cross_dq_kernel(CrossArgs a) {
     for (int x = 0; x < C::NSM; ++x) s[x] = dp[x] = f32x16{};
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
+      if (!in_dim<T>(16 * ks, a.dim)) break;
 #pragma unroll
       for (int x = 0; x < C::NSM; ++x) {
         s[x] = M::mul(ops.row(Ks, x, ks), qf[ks], s[x]);
@@ -176,8 +177,11 @@ void cross_dq_kernel(CrossArgs a) {
       // dS is rounded to T for the product, as P is for O
       const V8 bop = pack_op<T>(&ds[kk >> 1][8 * (kk & 1)]);
 #pragma unroll
-      for (int mt = 0; mt < D / 32; ++mt)
-        dq[mt] = M::mul(ops.col(Ks, 0, mt, kk), bop, dq[mt]), step_fence<T, D>();
+      for (int mt = 0; mt < D / 32; ++mt) {
+        if (!in_dim<T>(32 * mt, a.dim)) break;
+        dq[mt] = M::mul(ops.col(Ks, 0, mt, kk), bop, dq[mt]);
+        step_fence<T, D>();
+      }
     }
     dma_wait();
     __syncthreads();
@@ -251,13 +255,13 @@ void cross_dkv_kernel(CrossArgs a) {
   constexpr int DA = C::DA, HALVES = D / DA, KT = C::KT;
   __shared__ __attribute__((aligned(16))) char smem[C::NS * C::STAGE];
 
-  const int tile = xcd_tile(blockIdx.x, a.tiles * a.splits);
+  const int tile = tile_of(a);
   if (tile >= a.tiles * a.splits) return;
   const int split = tile % a.splits;
   int own = tile / a.splits;
   const int d0 = own % HALVES * DA;
   own /= HALVES;
-  const int hk = own / a.per_head;
+  const int hk = own / a.per_head;                  // batch * kv_heads + key head
   const int b = hk / a.kv_heads, kh = hk % a.kv_heads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 31, h = lane >> 5;
@@ -365,6 +369,7 @@ void cross_dkv_kernel(CrossArgs a) {
       f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
+        if (!in_dim<T>(16 * ks, a.dim)) break;
         s = M::mul(ops.row(Qs, 0, ks), kf[0][ks], s);
         dp = M::mul(ops.row(Gs, 0, ks), vf[0][ks], dp);
         step_fence<T, D>();
@@ -385,6 +390,7 @@ void cross_dkv_kernel(CrossArgs a) {
         const V8 pb = pack_op<T>(&p[8 * kk]), sb = pack_op<T>(&ds[8 * kk]);
 #pragma unroll
         for (int mt = 0; mt < DA / 32; ++mt) {
+          if (!in_dim<T>(d0 + 32 * mt, a.dim)) break;
           dv[mt][0] = M::mul(ops.col(Gs, d0, mt, kk), pb, dv[mt][0]);
           dk[mt][0] = M::mul(ops.col(Qs, d0, mt, kk), sb, dk[mt][0]);
           step_fence<T, D>();
@@ -601,23 +607,26 @@ int64_t splits_for(int64_t tiles, int64_t fit, int64_t steps, int64_t least) {
 // Splits of the pass over the queries.  With `fit` workgroups at once, s splits
 // take ceil(tiles s / fit) rounds of steps / s items and a workgroup's own cost
 // (about eight items: K and V in, the sums out), and their parts are written and
-// read again.
-int64_t dkv_splits(int64_t tiles, int64_t fit, int64_t steps, const Plan& p) {
+// read again.  Where samples may have fewer keys (`some`), half of the tiles
+// having no valid one counts as much as all of them at work.
+int64_t dkv_splits(int64_t tiles, int64_t fit, int64_t steps, int nw, bool some) {
   int64_t best = 1;
   double least = 1e300;
-  const double part = 0.05 * p.k_nw * (double)tiles / (double)fit;   // of an item's time
+  const double part = 0.2 * nw * (double)tiles / (double)fit;   // of an item's time
   for (int64_t s = 1; s <= 64 && s <= steps; ++s) {
     const int64_t per = (steps + s - 1) / s;
     if ((steps + per - 1) / per != s) continue;
-    const double rounds = (double)((tiles * s + fit - 1) / fit);
-    const double cost = rounds * (double)(per + 8) + (s > 1 ? 8 + part * 4 * (double)s : 0);
+    const double all = (double)((tiles * s + fit - 1) / fit);
+    const double half = (double)(((tiles + 1) / 2 * s + fit - 1) / fit);
+    const double cost = (some ? all + half : 2 * all) * (double)(per + 8) +
+                        (s > 1 ? 16 + 2 * part * (double)s : 0);
     if (cost < least) least = cost, best = s;
   }
   return best;
 }
 
 Plan bwd_plan(const vsa_cross* c) {
-  Plan p;
+  Plan p = {};
   const int64_t group = c->heads / c->kv_heads, rows = group * c->sq;
   const int es = c->dtype == VSA_F32 ? 4 : 2;
   p.kd = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
@@ -637,7 +646,8 @@ Plan bwd_plan(const vsa_cross* c) {
   const int stage = 2 * 32 * p.kd * es + 256;
   const int64_t kfit =
       (int64_t)cu_count() * std::max(1, std::min(160 * 1024 / (stage * (es == 2 ? 4 : 2)), 4 / p.k_nw));
-  p.k_splits = (int)dkv_splits(p.k_tiles, kfit, group * ((c->sq + 31) / 32), p);
+  p.k_splits = (int)dkv_splits(p.k_tiles, kfit, group * ((c->sq + 31) / 32), p.k_nw,
+                               c->batch > 1 && (c->kv_lens || c->key_mask));
   return p;
 }
 

@@ -39,14 +39,14 @@ void cross_fwd_kernel(CrossArgs a) {
   constexpr int KC = C::KC;
   __shared__ __attribute__((aligned(16))) char smem[2 * C::STAGE];
 
-  const int tile = xcd_tile(blockIdx.x, a.tiles * a.splits);
+  const int tile = tile_of(a);
   if (tile >= a.tiles * a.splits) return;
   const int split = tile % a.splits, own = tile / a.splits;
   const int hk = own / a.per_head;                  // batch * kv_heads + key head
   const int b = hk / a.kv_heads, kh = hk % a.kv_heads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 31, h = lane >> 5;
-  const int row = (own % a.per_head) * (32 * NW) + wave * 32 + r;  // of group * sq
+  const int row = own % a.per_head * (32 * NW) + wave * 32 + r;  // of group * sq
   const int rows = a.group * a.sq;
   const int at = min(row, rows - 1);
   const int head = kh * a.group + at / a.sq, sq_i = at % a.sq;
@@ -126,6 +126,7 @@ void cross_fwd_kernel(CrossArgs a) {
     for (int x = 0; x < C::NSM; ++x) sacc[x] = f32x16{};
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
+      if (!in_dim<T>(16 * ks, a.dim)) break;
 #pragma unroll
       for (int x = 0; x < C::NSM; ++x) sacc[x] = M::mul(ops.row(Ks, x, ks), qf[ks], sacc[x]);
       step_fence<T, D>();
@@ -166,8 +167,11 @@ void cross_fwd_kernel(CrossArgs a) {
     for (int kk = 0; kk < 2 * C::NSM; ++kk) {
       const V8 bop = pack_op<T>(&p[kk >> 1][8 * (kk & 1)]);
 #pragma unroll
-      for (int mt = 0; mt < D / 32; ++mt)
-        oacc[mt] = M::mul(ops.col(Vs, 0, mt, kk), bop, oacc[mt]), step_fence<T, D>();
+      for (int mt = 0; mt < D / 32; ++mt) {
+        if (!in_dim<T>(32 * mt, a.dim)) break;
+        oacc[mt] = M::mul(ops.col(Vs, 0, mt, kk), bop, oacc[mt]);
+        step_fence<T, D>();
+      }
     }
     dma_wait();
     __syncthreads();

@@ -61,10 +61,10 @@ def _three(x: Tensor) -> bytes:
 
 
 @functools.lru_cache(maxsize=256)
-def _sizes(b, h, hk, sq, skv, d, masked, dtype):
+def _sizes(b, h, hk, sq, skv, d, lens, masked, dtype):
     """Bytes of (forward scratch, backward scratch)."""
     # a pointer's presence is all that is read
-    c = _lib.CROSS.pack(256, 256, 256, 0, 256 if masked else 0, *(0, 0, 256) * 3, 0, sq, skv, b, h,
+    c = _lib.CROSS.pack(256, 256, 256, 256 if lens else 0, 256 if masked else 0, *(0, 0, 256) * 3, 0, sq, skv, b, h,
                         hk, d, dtype, 1.0)
     n = (ctypes.c_int64 * 2)()
     at = ctypes.addressof(n)
@@ -72,10 +72,10 @@ def _sizes(b, h, hk, sq, skv, d, masked, dtype):
     return tuple(n)
 
 
-def _scratch(q, k, masked: bool, which: int) -> Optional[Tensor]:
+def _scratch(q, k, lens, mask, which: int) -> Optional[Tensor]:
     b, h, sq, d = q.shape
-    return _workspace(_sizes(b, h, k.shape[1], sq, k.shape[2], d, masked,
-                             _lib.DTYPE_CODES[q.dtype])[which], q.device)
+    return _workspace(_sizes(b, h, k.shape[1], sq, k.shape[2], d, lens is not None,
+                             mask is not None, _lib.DTYPE_CODES[q.dtype])[which], q.device)
 
 
 def _forward(q, k, v, lens, mask, scale, keep):
@@ -88,7 +88,7 @@ def _forward(q, k, v, lens, mask, scale, keep):
             lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
             if q.dtype != torch.float32:
                 lo = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        scratch = _scratch(q, k, mask is not None, 0)
+        scratch = _scratch(q, k, lens, mask, 0)
         _lib.call("vsa_cross_fwd", _pack(q, k, v, lens, mask, scale), out.data_ptr(), _three(out),
                   _ptr(lo), _ptr(lse), _ptr(scratch),
                   torch._C._cuda_getCurrentRawStream(dev.index))
@@ -102,7 +102,7 @@ def _backward(q, k, v, lens, mask, scale, out, lo, lse, dout):
         q, k, v, out, dout = (_rows16(x) for x in (q, k, v, out, dout))
         lo = lo if lo is None else _rows16(lo.contiguous())
         dq, dk, dv = (empty_in_order(x) for x in (q, k, v))
-        scratch = _scratch(q, k, mask is not None, 1)
+        scratch = _scratch(q, k, lens, mask, 1)
         _lib.call("vsa_cross_bwd", _pack(q, k, v, lens, mask, scale), out.data_ptr(), _three(out),
                   _ptr(lo), dout.data_ptr(), _three(dout), lse.data_ptr(), dq.data_ptr(),
                   _three(dq), dk.data_ptr(), _three(dk), dv.data_ptr(), _three(dv), _ptr(scratch),

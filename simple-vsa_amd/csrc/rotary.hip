@@ -113,13 +113,17 @@ __device__ __forceinline__ void st_piece(T* p, const Piece<T, V>& v) {
     *reinterpret_cast<Piece<T, V>*>(p) = v;
 }
 
-// A thread owns V pairs of one token (two pieces of V channels) and walks the
-// heads of q and k with their cosines and sines in registers, so the table is
-// read once a token and not once a head.  A unit behind the turned channels
-// copies V channels.
-template <typename T, int V, bool INTER>
+// A thread owns a unit of one token's channels, the same in every head, and walks
+// the heads of q and k with its cosines and sines in registers, so the table is
+// read once a token and not once a head.  A unit is V pairs in two pieces of V
+// channels, or with INTER V / 2 pairs in one piece (two pieces a thread left each
+// load instruction on every other 16 bytes: 24 heads x 16k tokens 61 -> TIME us),
+// or behind the turned channels a piece that is copied.  LOOSE: no alignment but
+// the element's (INTER with an odd start or end: elements one by one).
+template <typename T, int V, bool INTER, bool LOOSE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-  const int per = 256 / a.units;   // tokens of a workgroup
+  constexpr int P = INTER ? V / 2 : V;   // pairs of a unit
+  const int per = 256 / a.units;         // tokens of a workgroup
   const int unit = threadIdx.x % a.units;
   if ((int)threadIdx.x >= per * a.units) return;
   int64_t g = blockIdx.x;
@@ -130,12 +134,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   const int64_t t = g % blocks * per + threadIdx.x / a.units;
   if (t >= a.tokens) return;
   const bool turn = unit < a.turns;
-  const int o1 = !turn ? 2 * a.pairs + (unit - a.turns) * V : INTER ? 2 * unit * V : unit * V;
-  const int o2 = INTER ? o1 + V : a.pairs + o1;
+  const int o1 = turn ? unit * V : 2 * a.pairs + (unit - a.turns) * V;
+  const int o2 = a.pairs + o1;           // the second piece, without INTER
 
-  float c[V], s[V];
+  float c[P], s[P];
 #pragma unroll
-  for (int e = 0; e < V; ++e) c[e] = 1.f, s[e] = 0.f;
+  for (int e = 0; e < P; ++e) c[e] = 1.f, s[e] = 0.f;
   if (turn) {
     int64_t p = t;
     if (a.positions) {
@@ -144,14 +148,28 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     }
     if (p >= a.rows) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) c[e] = s[e] = NAN;
+      for (int e = 0; e < P; ++e) c[e] = s[e] = NAN;
     } else if (p >= 0) {
-      const float* cp = a.co + p * a.pairs + unit * V;
-      const float* sp = a.si + p * a.pairs + unit * V;
+      const float* cp = a.co + p * a.pairs + unit * P;
+      const float* sp = a.si + p * a.pairs + unit * P;
 #pragma unroll
-      for (int e = 0; e < V; ++e) c[e] = cp[e], s[e] = sp[e] * a.sign;
+      for (int e = 0; e < P; ++e) c[e] = cp[e], s[e] = sp[e] * a.sign;
     }
   }
+  auto load = [&](const T* x) {
+    if constexpr (!LOOSE) return ld_piece<T, V>(x);
+    Piece<T, V> r;
+    const int64_t left = a.dim - o1;
+#pragma unroll
+    for (int e = 0; e < V; ++e) r.e[e] = x[e < left ? e : 0];
+    return r;
+  };
+  auto store = [&](T* y, const Piece<T, V>& v) {
+    if constexpr (!LOOSE) return st_piece<T, V>(y, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < a.dim - o1) y[e] = v.e[e];
+  };
   const int h0 = hb * a.per_block, h1 = min(h0 + a.per_block, a.heads);
   constexpr int UR = 4;
   for (int h = h0; h < h1; h += UR) {
@@ -162,63 +180,51 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
       const int w = hh >= a.heads_q;
       const T* x = (const T*)a.x[w] + b * a.xs[w][0] + (hh - w * a.heads_q) * a.xs[w][1] +
                    t * a.xs[w][2];
-      x1[u] = ld_piece<T, V>(x + o1);
-      if (turn) x2[u] = ld_piece<T, V>(x + o2);
+      x1[u] = load(x + o1);
+      if (!INTER && turn) x2[u] = load(x + o2);
     }
 #pragma unroll
     for (int u = 0; u < UR; ++u) {
       if (h + u >= h1) break;
       const int w = h + u >= a.heads_q;
       T* y = (T*)a.y[w] + b * a.ys[w][0] + (h + u - w * a.heads_q) * a.ys[w][1] + t * a.ys[w][2];
-      if (!turn) {
-        st_piece<T, V>(y + o1, x1[u]);
-        continue;
-      }
-      Piece<T, V> y1, y2;
+      if (turn) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        // the pair e of this unit: element e of both pieces, or elements 2e and
-        // 2e + 1 of the two in a row
-        const float p = Elem<T>::to_f(!INTER ? x1[u].e[e] : 2 * e < V ? x1[u].e[2 * e]
-                                                                     : x2[u].e[2 * e - V]);
-        const float q = Elem<T>::to_f(!INTER ? x2[u].e[e] : 2 * e + 1 < V ? x1[u].e[2 * e + 1]
-                                                                         : x2[u].e[2 * e + 1 - V]);
-        const T r1 = Elem<T>::from_f(p * c[e] - q * s[e]);
-        const T r2 = Elem<T>::from_f(q * c[e] + p * s[e]);
-        if (!INTER) {
-          y1.e[e] = r1;
-          y2.e[e] = r2;
-        } else {
-          (2 * e < V ? y1.e[2 * e] : y2.e[2 * e - V]) = r1;
-          (2 * e + 1 < V ? y1.e[2 * e + 1] : y2.e[2 * e + 1 - V]) = r2;
+        for (int e = 0; e < P; ++e) {
+          T& lo = INTER ? x1[u].e[2 * e] : x1[u].e[e];
+          T& hi = INTER ? x1[u].e[2 * e + 1] : x2[u].e[e];
+          const float p = Elem<T>::to_f(lo), q = Elem<T>::to_f(hi);
+          lo = Elem<T>::from_f(p * c[e] - q * s[e]);
+          hi = Elem<T>::from_f(q * c[e] + p * s[e]);
         }
+        if (!INTER) store(y + o2, x2[u]);
       }
-      st_piece<T, V>(y + o1, y1);
-      st_piece<T, V>(y + o2, y2);
+      store(y + o1, x1[u]);
     }
   }
 }
 
-template <typename T, int V>
-static int launch_rotary(const RotaryArgs& a, int64_t batch, bool inter, hipStream_t s) {
+template <typename T, int V, bool INTER, bool LOOSE = false>
+static int launch_rotary(const RotaryArgs& a, int64_t batch, hipStream_t s) {
   const int per = 256 / a.units;
   const int64_t grid = (a.tokens + per - 1) / per * batch * a.head_blocks;
   if (grid > (1LL << 31) - 1) return VSA_ERR_SHAPE;
-  if (inter)
-    hipLaunchKernelGGL((rotary_kernel<T, V, true>), dim3((unsigned)grid), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((rotary_kernel<T, V, false>), dim3((unsigned)grid), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((rotary_kernel<T, V, INTER, LOOSE>), dim3((unsigned)grid), dim3(256), 0, s, a);
   return vsa_check_launch();
 }
 
+// v: channels of a piece that every start and length allows
 template <typename T>
 static int rotary_of(const RotaryArgs& a, int64_t batch, int v, bool inter, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (v == 8) return launch_rotary<T, 8>(a, batch, inter, s);
+    if (v == 8)
+      return inter ? launch_rotary<T, 8, true>(a, batch, s) : launch_rotary<T, 8, false>(a, batch, s);
   }
-  if (v == 4) return launch_rotary<T, 4>(a, batch, inter, s);
-  if (v == 2) return launch_rotary<T, 2>(a, batch, inter, s);
-  return launch_rotary<T, 1>(a, batch, inter, s);
+  if (v == 4)
+    return inter ? launch_rotary<T, 4, true>(a, batch, s) : launch_rotary<T, 4, false>(a, batch, s);
+  if (v == 2)
+    return inter ? launch_rotary<T, 2, true>(a, batch, s) : launch_rotary<T, 2, false>(a, batch, s);
+  return inter ? launch_rotary<T, 2, true, true>(a, batch, s) : launch_rotary<T, 1, false>(a, batch, s);
 }
 
 }  // namespace vsa
@@ -294,7 +300,9 @@ extern "C" int vsa_rotary(const vsa_rotary_op* op, void* stream) {
   RotaryArgs a;
   a.x[0] = op->q, a.x[1] = op->k, a.y[0] = op->q_out, a.y[1] = op->k_out;
   // the widest pieces that every row's start and every piece of a row allow
-  uint64_t low = (uint64_t)op->channels / 2 | (uint64_t)(op->head_dim - op->channels) | 8;
+  const bool inter = op->interleaved != 0;
+  uint64_t low = (uint64_t)(inter ? op->channels : op->channels / 2) |
+                 (uint64_t)(op->head_dim - op->channels) | 8;
   for (int w = 0; w < (op->k_heads ? 2 : 1); ++w) {
     low |= ((uint64_t)a.x[w] | (uint64_t)a.y[w]) / es;
     if (((uintptr_t)a.x[w] | (uintptr_t)a.y[w]) % es) return VSA_ERR_ALIGN;
@@ -314,8 +322,9 @@ extern "C" int vsa_rotary(const vsa_rotary_op* op, void* stream) {
   a.rows = op->rows, a.tokens = op->tokens;
   a.heads_q = op->q_heads, a.heads = op->q_heads + op->k_heads;
   a.dim = op->head_dim, a.pairs = op->channels / 2;
-  a.turns = a.pairs / v;
-  a.units = a.turns + (op->head_dim - op->channels) / v;
+  const int unit = inter && v == 1 ? 2 : v;
+  a.turns = (inter ? op->channels : a.pairs) / unit;
+  a.units = a.turns + (op->head_dim - op->channels + unit - 1) / unit;
   a.sign = op->inverse ? -1.f : 1.f;
   const int per = 256 / a.units;
   const int64_t blocks = (a.tokens + per - 1) / per * op->batch;
@@ -325,6 +334,5 @@ extern "C" int vsa_rotary(const vsa_rotary_op* op, void* stream) {
   a.per_block = (int)((a.heads + split - 1) / split);
   a.head_blocks = (a.heads + a.per_block - 1) / a.per_block;
   hipStream_t s = (hipStream_t)stream;
-  const bool inter = op->interleaved != 0;
   VSA_DISPATCH_ALL(op->dtype, T, return rotary_of<T>(a, op->batch, v, inter, s));
 }

@@ -33,6 +33,8 @@ def _rows16(x: Tensor) -> Tensor:
     """x itself where the kernels read its rows in place (channels next to each
     other, every row 16-byte aligned, a tile's rows within reach of a 32-bit
     offset), else a dense copy."""
+    if x.is_contiguous():
+        return x if x.data_ptr() % 16 == 0 else x.clone()
     es = x.element_size()
     if x.stride(3) == 1 and x.data_ptr() % 16 == 0:
         b, h, s = _strides(x)

@@ -10,6 +10,7 @@ Nothing here runs on the CPU: a CPU tensor or a missing kernel library raises.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple, Union
 
@@ -35,6 +36,38 @@ def _three(x, name, kind=float) -> Tuple:
     return tuple(kind(v) for v in x)
 
 
+@functools.lru_cache(maxsize=64)
+def _axes(shape, channels, theta, start, factor, method, original):
+    """(the axes' structs, tokens, pairs) of checked arguments."""
+    if min(shape) <= 0:
+        raise ValueError("dit_seq_shape must be positive")
+    if math.prod(shape) >= 1 << 31:
+        raise ValueError("a rotary table holds fewer than 2^31 tokens")
+    if min(channels) < 0 or any(c % 2 for c in channels) or not \
+            0 < sum(channels) <= MAX_ROTARY_CHANNELS:
+        raise ValueError("axis_channels must be even, and together in "
+                         f"[2, {MAX_ROTARY_CHANNELS}]")
+    if not (theta > 0 and math.isfinite(theta)):
+        raise ValueError("theta must be positive and finite")
+    if not all(f > 0 and math.isfinite(f) for f in factor):
+        raise ValueError("factor must be positive and finite")
+    if not all(abs(x) <= 2.0 ** 52 for x in start):
+        raise ValueError("start must lie within 2^52")
+    if method not in ROTARY_METHODS:
+        raise ValueError(f"method must be one of {ROTARY_METHODS}")
+    if method == "yarn":
+        if original is None:
+            raise ValueError("the yarn method needs original_shape, the trained (T, H, W)")
+        if not all(x > 0 and math.isfinite(x) for x in original):
+            raise ValueError("original_shape must be positive")
+    else:
+        original = (0.0,) * 3
+    kind = ROTARY_METHODS.index(method)
+    axes = _lib.ROTARY_AXES.pack(*(x for i in range(3) for x in (
+        shape[i], channels[i], kind, 0, start[i], theta, factor[i], original[i])))
+    return axes, math.prod(shape), sum(channels) // 2
+
+
 def build_rotary_table(dit_seq_shape: Tuple[int, int, int], axis_channels: Tuple[int, int, int],
                        theta: float = 10000.0, *, start=(0, 0, 0),
                        factor: Union[float, Tuple[float, float, float]] = 1.0,
@@ -51,42 +84,16 @@ def build_rotary_table(dit_seq_shape: Tuple[int, int, int], axis_channels: Tuple
     that turn 32 times or more in ``original_shape`` (the trained sizes), divides
     those that turn once or less, a ramp between, and multiplies cos and sin by
     ``0.1 ln(factor) + 1``.  Angles are made in 64 bits."""
-    shape = _three(dit_seq_shape, "dit_seq_shape", int)
-    channels = _three(axis_channels, "axis_channels", int)
-    start, factor = _three(start, "start"), _three(factor, "factor")
-    if min(shape) <= 0:
-        raise ValueError("dit_seq_shape must be positive")
-    if math.prod(shape) >= 1 << 31:
-        raise ValueError("a rotary table holds fewer than 2^31 tokens")
-    if min(channels) < 0 or any(c % 2 for c in channels) or not \
-            0 < sum(channels) <= MAX_ROTARY_CHANNELS:
-        raise ValueError("axis_channels must be even, and together in "
-                         f"[2, {MAX_ROTARY_CHANNELS}]")
-    theta = float(theta)
-    if not (theta > 0 and math.isfinite(theta)):
-        raise ValueError("theta must be positive and finite")
-    if not all(f > 0 and math.isfinite(f) for f in factor):
-        raise ValueError("factor must be positive and finite")
-    if not all(abs(x) <= 2.0 ** 52 for x in start):
-        raise ValueError("start must lie within 2^52")
-    if method not in ROTARY_METHODS:
-        raise ValueError(f"method must be one of {ROTARY_METHODS}")
-    original = (0.0,) * 3
-    if method == "yarn":
-        if original_shape is None:
-            raise ValueError("the yarn method needs original_shape, the trained (T, H, W)")
-        original = _three(original_shape, "original_shape")
-        if not all(x > 0 and math.isfinite(x) for x in original):
-            raise ValueError("original_shape must be positive")
+    axes, tokens, pairs = _axes(
+        _three(dit_seq_shape, "dit_seq_shape", int), _three(axis_channels, "axis_channels", int),
+        float(theta), _three(start, "start"), _three(factor, "factor"), method,
+        None if original_shape is None else _three(original_shape, "original_shape"))
     device = torch.device(device)
     if device.type != "cuda":
         raise ValueError("the MI355X implementation requires a GPU device")
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    kind = ROTARY_METHODS.index(method)
-    axes = _lib.ROTARY_AXES.pack(*(x for i in range(3) for x in (
-        shape[i], channels[i], kind, 0, start[i], theta, factor[i], original[i])))
-    cos = torch.empty((math.prod(shape), sum(channels) // 2), dtype=torch.float32, device=device)
+    cos = torch.empty((tokens, pairs), dtype=torch.float32, device=device)
     sin = torch.empty_like(cos)
     with on_device(device):
         _lib.call("vsa_rotary_table", axes, cos.data_ptr(), sin.data_ptr(),
@@ -104,9 +111,11 @@ def token_order(x: Tensor) -> bool:
     return x.shape[1] > 1 and x.shape[2] > 1 and x.stride(1) < x.stride(2)
 
 
-def empty_in_order(x: Tensor, shape=None) -> Tensor:
-    """An uninitialised [B, H, S, D] tensor, dense, in x's order of heads and tokens."""
-    b, h, s, d = x.shape if shape is None else shape
+def empty_in_order(x: Tensor) -> Tensor:
+    """An uninitialised tensor of x's shape, dense, in x's order of heads and tokens."""
+    if x.is_contiguous():
+        return torch.empty_like(x)
+    b, h, s, d = x.shape
     if token_order(x):
         return torch.empty((b, s, h, d), dtype=x.dtype, device=x.device).transpose(1, 2)
     return torch.empty((b, h, s, d), dtype=x.dtype, device=x.device)
@@ -157,13 +166,18 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, gq, gk):
         cos, sin, positions = ctx.saved_tensors
         interleaved, inverse = ctx.options
-        got = [g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad)]
-        live = [g for g in got if g is not None]
-        if live:
-            rest = (cos, sin, positions, interleaved, not inverse)
-            turned = iter(_Rotary.apply(live[0], live[1] if len(live) > 1 else None, *rest))
-            got = [None if g is None else next(turned) for g in got]
-        return (*got, None, None, None, None, None)
+        if not ctx.needs_input_grad[0]:
+            gq = None
+        if not ctx.needs_input_grad[1]:
+            gk = None
+        # through autograd again only where a second derivative may be wanted
+        turn = _Rotary.apply if torch.is_grad_enabled() else _rotate
+        if gq is None:
+            if gk is not None:
+                gk = turn(gk, None, cos, sin, positions, interleaved, not inverse)[0]
+        else:
+            gq, gk = turn(gq, gk, cos, sin, positions, interleaved, not inverse)
+        return gq, gk, None, None, None, None, None
 
 
 def _check_rotary(q, k, cos, sin, positions) -> None:

@@ -23,11 +23,11 @@ constexpr float kSlack = 8.0f;  // log2 units
 template <typename T, int D, int NW>
 struct CrossFwdCfg {
   static constexpr int NT = NW * 64;
-  static constexpr int KC = sizeof(T) == 2 && D <= 128 && NW == 4 ? 64 : 32;
+  static constexpr int KC = sizeof(T) == 2 && D < 128 && NW == 4 ? 64 : 32;
   static constexpr int NSM = KC / 32;
   static constexpr int TILE = KC * D * (int)sizeof(T);   // bytes of a K (or V) chunk
   static constexpr int STAGE = 2 * TILE;
-  static constexpr int WPE = D * (int)sizeof(T) > 256 ? 1 : 2;
+  static constexpr int WPE = D * (int)sizeof(T) > 256 ? 1 : sizeof(T) == 2 ? 3 : 2;
 };
 
 template <typename T, int D, int NW>
@@ -529,7 +529,7 @@ struct Plan {
 };
 
 int fwd_kc(const vsa_cross* c, int kd, int nw) {
-  return c->dtype != VSA_F32 && kd <= 128 && nw == 4 ? 64 : 32;
+  return c->dtype != VSA_F32 && kd < 128 && nw == 4 ? 64 : 32;
 }
 
 Plan fwd_plan(const vsa_cross* c) {

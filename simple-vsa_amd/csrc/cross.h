@@ -52,6 +52,17 @@ __device__ __forceinline__ typename Mma<T>::V8 pack_op(const float* v) {
   }
 }
 
+// Eight values as an operand, and what rounding them to T left over as another.
+template <typename T>
+__device__ __forceinline__ void pack_both(const float* v, typename Mma<T>::V8& hi,
+                                          typename Mma<T>::V8& lo) {
+  hi = pack_op<T>(v);
+  float rest[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) rest[e] = v[e] - (float)hi[e];
+  lo = pack_op<T>(rest);
+}
+
 // 8 consecutive elements at a 16-byte aligned address
 template <typename T>
 __device__ __forceinline__ typename Mma<T>::V8 ld8(const T* p) {

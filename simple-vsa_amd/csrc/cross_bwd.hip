@@ -22,11 +22,11 @@ namespace vsa {
 template <typename T, int D, int NW>
 struct CrossDqCfg {
   static constexpr int NT = NW * 64;
-  static constexpr int KC = sizeof(T) == 2 && D == 64 && NW == 4 ? 64 : 32;
+  static constexpr int KC = 32;
   static constexpr int NSM = KC / 32;
   static constexpr int TILE = KC * D * (int)sizeof(T);
   static constexpr int STAGE = 2 * TILE;
-  static constexpr int WPE = D * (int)sizeof(T) > 256 ? 1 : 2;
+  static constexpr int WPE = D * (int)sizeof(T) > 256 ? 1 : D == 64 && sizeof(T) == 2 ? 3 : 2;
 };
 
 template <typename T, int D, int NW>
@@ -50,6 +50,35 @@ void cross_dq_kernel(CrossArgs a) {
   const int at = min(row, rows - 1);
   const int head = kh * a.group + at / a.sq, sq_i = at % a.sq;
   const int64_t stat = ((int64_t)b * a.heads + head) * a.sq + sq_i;
+
+  const T* kbase = (const T*)a.k.p + b * a.k.b + kh * a.k.h;
+  const T* vbase = (const T*)a.v.p + b * a.v.b + kh * a.v.h;
+  TileCopy<T, D, KC, C::NT> kcopy, vcopy;
+  kcopy.init(a.k.s, a.dim, threadIdx.x);
+  vcopy.init(a.v.s, a.dim, threadIdx.x);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem));
+  Operands<T, D> ops;
+  ops.init(smem, r, h);
+  const int chunks = (a.skv + KC - 1) / KC;
+  const int per_split = (chunks + a.splits - 1) / a.splits;
+  KeyWalk<KC> walk;
+  walk.init(a, b, split * per_split, per_split);
+  auto copy = [&](int stage) __attribute__((always_inline)) {
+    const int left = walk.n - walk.j * KC;
+    const auto ks = kcopy.rows(kbase + (int64_t)walk.j * KC * a.k.s, left);
+    const auto vs = vcopy.rows(vbase + (int64_t)walk.j * KC * a.v.s, left);
+    const uint32_t to = lds0 + stage * C::STAGE;
+    if (!walk.holes()) {
+      kcopy.copy(to, ks);
+      vcopy.copy(to + C::TILE, vs);
+    } else {
+      kcopy.copy_valid(to, ks, walk.w);
+      vcopy.copy_valid(to + C::TILE, vs, walk.w);
+    }
+  };
+
+  bool have = walk.find();
+  if (have) copy(0);   // in flight with the rows' loads
 
   V8 qf[D / 16], gf[D / 16];
   float delta = 0.f;
@@ -103,37 +132,9 @@ void cross_dq_kernel(CrossArgs a) {
   if (store && h == 0 && split == 0) a.delta[stat] = delta;
   const float lse = a.lse[stat];
 
-  const T* kbase = (const T*)a.k.p + b * a.k.b + kh * a.k.h;
-  const T* vbase = (const T*)a.v.p + b * a.v.b + kh * a.v.h;
-  TileCopy<T, D, KC, C::NT> kcopy, vcopy;
-  kcopy.init(a.k.s, a.dim, threadIdx.x);
-  vcopy.init(a.v.s, a.dim, threadIdx.x);
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem));
-  Operands<T, D> ops;
-  ops.init(smem, r, h);
-  const int chunks = (a.skv + KC - 1) / KC;
-  const int per_split = (chunks + a.splits - 1) / a.splits;
-  KeyWalk<KC> walk;
-  walk.init(a, b, split * per_split, per_split);
-  auto copy = [&](int stage) __attribute__((always_inline)) {
-    const int left = walk.n - walk.j * KC;
-    const auto ks = kcopy.rows(kbase + (int64_t)walk.j * KC * a.k.s, left);
-    const auto vs = vcopy.rows(vbase + (int64_t)walk.j * KC * a.v.s, left);
-    const uint32_t to = lds0 + stage * C::STAGE;
-    if (!walk.holes()) {
-      kcopy.copy(to, ks);
-      vcopy.copy(to + C::TILE, vs);
-    } else {
-      kcopy.copy_valid(to, ks, walk.w);
-      vcopy.copy_valid(to + C::TILE, vs, walk.w);
-    }
-  };
-
   f32x16 dq[D / 32];
 #pragma unroll
   for (int mt = 0; mt < D / 32; ++mt) dq[mt] = f32x16{};
-  bool have = walk.find();
-  if (have) copy(0);
   dma_wait();
   __syncthreads();
   auto chunk = [&](auto stage_c) __attribute__((always_inline)) {
@@ -174,12 +175,17 @@ void cross_dq_kernel(CrossArgs a) {
     }
 #pragma unroll
     for (int kk = 0; kk < 2 * C::NSM; ++kk) {
-      // dS is rounded to T for the product, as P is for O
-      const V8 bop = pack_op<T>(&ds[kk >> 1][8 * (kk & 1)]);
+      // dS as T and what that leaves over: rounded once, a third more of this
+      // pass' products less, dQ is further off than its own rounding makes it
+      // (bf16, 512 keys: 2.5e-3 of its norm against 1.7e-3)
+      V8 hi, lo;
+      pack_both<T>(&ds[kk >> 1][8 * (kk & 1)], hi, lo);
 #pragma unroll
       for (int mt = 0; mt < D / 32; ++mt) {
         if (!in_dim<T>(32 * mt, a.dim)) break;
-        dq[mt] = M::mul(ops.col(Ks, 0, mt, kk), bop, dq[mt]);
+        const V8 k = ops.col(Ks, 0, mt, kk);
+        dq[mt] = M::mul(k, hi, dq[mt]);
+        if constexpr (sizeof(T) == 2) dq[mt] = M::mul(k, lo, dq[mt]);
         step_fence<T, D>();
       }
     }
@@ -607,19 +613,22 @@ int64_t splits_for(int64_t tiles, int64_t fit, int64_t steps, int64_t least) {
 // Splits of the pass over the queries.  With `fit` workgroups at once, s splits
 // take ceil(tiles s / fit) rounds of steps / s items and a workgroup's own cost
 // (about eight items: K and V in, the sums out), and their parts are written and
-// read again.  Where samples may have fewer keys (`some`), half of the tiles
-// having no valid one counts as much as all of them at work.
-int64_t dkv_splits(int64_t tiles, int64_t fit, int64_t steps, int nw, bool some) {
+// read again.  Where samples may have fewer keys (`some`), a quarter and a half of
+// the tiles having no valid one count as much as all of them at work.
+int64_t dkv_splits(int64_t tiles, int64_t fit, int64_t steps, int nw, int es, bool some) {
   int64_t best = 1;
   double least = 1e300;
-  const double part = 0.2 * nw * (double)tiles / (double)fit;   // of an item's time
+  // writing and reading a part takes 0.01 items' time for each wave's keys; an
+  // fp32 item takes eight times a 16-bit one's time
+  const double item = es == 2 ? 1 : 8, part = 0.01 * nw * (double)tiles / item;
   for (int64_t s = 1; s <= 64 && s <= steps; ++s) {
     const int64_t per = (steps + s - 1) / s;
     if ((steps + per - 1) / per != s) continue;
-    const double all = (double)((tiles * s + fit - 1) / fit);
-    const double half = (double)(((tiles + 1) / 2 * s + fit - 1) / fit);
-    const double cost = (some ? all + half : 2 * all) * (double)(per + 8) +
-                        (s > 1 ? 16 + 2 * part * (double)s : 0);
+    double rounds = 0;
+    for (int live = 4; live >= (some ? 2 : 4); --live)
+      rounds += (double)(((tiles * live + 3) / 4 * s + fit - 1) / fit);
+    if (some) rounds /= 3;
+    const double cost = rounds * ((double)per + 8 / item) + (s > 1 ? 8 / item + part * (double)s : 0);
     if (cost < least) least = cost, best = s;
   }
   return best;
@@ -636,7 +645,7 @@ Plan bwd_plan(const vsa_cross* c) {
   p.q_nw = rows <= 32 && !wide ? 1 : rows <= 64 ? 2 : 4;
   p.q_per_head = (int)((rows + 32 * p.q_nw - 1) / (32 * p.q_nw));
   p.q_tiles = (int64_t)c->batch * c->kv_heads * p.q_per_head;
-  const int lds = 4 * (es == 2 && p.kd == 64 && p.q_nw == 4 ? 64 : 32) * p.kd * es;
+  const int lds = 4 * 32 * p.kd * es;
   const int64_t fit = (int64_t)cu_count() * std::max(1, std::min(160 * 1024 / lds, 8 / p.q_nw));
   p.q_splits = (int)splits_for(p.q_tiles, fit, (c->skv + 31) / 32, 4);
   const int wave_keys = es == 2 && p.kd == 64 ? 64 : 32;
@@ -646,7 +655,7 @@ Plan bwd_plan(const vsa_cross* c) {
   const int stage = 2 * 32 * p.kd * es + 256;
   const int64_t kfit =
       (int64_t)cu_count() * std::max(1, std::min(160 * 1024 / (stage * (es == 2 ? 4 : 2)), 4 / p.k_nw));
-  p.k_splits = (int)dkv_splits(p.k_tiles, kfit, group * ((c->sq + 31) / 32), p.k_nw,
+  p.k_splits = (int)dkv_splits(p.k_tiles, kfit, group * ((c->sq + 31) / 32), p.k_nw, es,
                                c->batch > 1 && (c->kv_lens || c->key_mask));
   return p;
 }

@@ -51,26 +51,6 @@ void cross_fwd_kernel(CrossArgs a) {
   const int at = min(row, rows - 1);
   const int head = kh * a.group + at / a.sq, sq_i = at % a.sq;
 
-  V8 qf[D / 16];
-  {
-    const T* qrow = (const T*)a.q.p + b * a.q.b + head * a.q.h + sq_i * a.q.s;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      const int d = 16 * ks + 8 * h;
-      V8 x = zero8<T>();
-      if (d < a.dim) x = ld8<T>(qrow + d);
-      // a negative softmax scale is folded into q (the sign bit of each element)
-      if constexpr (sizeof(T) == 2) {
-        u32x4 raw = __builtin_bit_cast(u32x4, x);
-        raw ^= a.qsign;
-        qf[ks] = as_vec8<T>(raw);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(__float_as_uint(x[e]) ^ a.qsign);
-        qf[ks] = x;
-      }
-    }
-  }
   const T* kbase = (const T*)a.k.p + b * a.k.b + kh * a.k.h;
   const T* vbase = (const T*)a.v.p + b * a.v.b + kh * a.v.h;
   TileCopy<T, D, KC, C::NT> kcopy, vcopy;
@@ -98,14 +78,35 @@ void cross_fwd_kernel(CrossArgs a) {
     }
   };
 
+  bool have = walk.find();
+  const bool any = have;
+  if (have) copy(0);   // in flight with the rows' loads
+
+  V8 qf[D / 16];
+  {
+    const T* qrow = (const T*)a.q.p + b * a.q.b + head * a.q.h + sq_i * a.q.s;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const int d = 16 * ks + 8 * h;
+      V8 x = zero8<T>();
+      if (d < a.dim) x = ld8<T>(qrow + d);
+      // a negative softmax scale is folded into q (the sign bit of each element)
+      if constexpr (sizeof(T) == 2) {
+        u32x4 raw = __builtin_bit_cast(u32x4, x);
+        raw ^= a.qsign;
+        qf[ks] = as_vec8<T>(raw);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(__float_as_uint(x[e]) ^ a.qsign);
+        qf[ks] = x;
+      }
+    }
+  }
   float m = -INFINITY, lsum = 0.f;
   f32x16 oacc[D / 32];
 #pragma unroll
   for (int mt = 0; mt < D / 32; ++mt) oacc[mt] = f32x16{};
 
-  bool have = walk.find();
-  const bool any = have;
-  if (have) copy(0);
   dma_wait();
   __syncthreads();
   // one chunk, of stage `stage` (a constant: every LDS address is a lane offset

@@ -85,6 +85,7 @@ def _forward(q, k, v, lens, mask, scale, keep):
     dev = q.device
     with on_device(dev):
         out = empty_in_order(q)
+        q, k, v = _rows16(q), _rows16(k), _rows16(v)
         lo = lse = None
         if keep:
             lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
@@ -100,10 +101,10 @@ def _forward(q, k, v, lens, mask, scale, keep):
 def _backward(q, k, v, lens, mask, scale, out, lo, lse, dout):
     dev = q.device
     with on_device(dev):
+        dq, dk, dv = (empty_in_order(x) for x in (q, k, v))
         # (the saved ones too: a saved-tensor hook may give back other addresses)
         q, k, v, out, dout = (_rows16(x) for x in (q, k, v, out, dout))
         lo = lo if lo is None else _rows16(lo.contiguous())
-        dq, dk, dv = (empty_in_order(x) for x in (q, k, v))
         scratch = _scratch(q, k, lens, mask, 1)
         _lib.call("vsa_cross_bwd", _pack(q, k, v, lens, mask, scale), out.data_ptr(), _three(out),
                   _ptr(lo), dout.data_ptr(), _three(dout), lse.data_ptr(), dq.data_ptr(),
@@ -196,8 +197,8 @@ def mi355x_cross_attention(q: Tensor, k: Tensor, v: Tensor, kv_lens: Optional[Te
         mask = mask.contiguous()
     if d % 8:   # rows of whole 16-byte pieces; zero channels change no product
         q, k, v = (torch.nn.functional.pad(x, (0, 8 - d % 8)) for x in (q, k, v))
-    q, k, v = (_rows16(x) for x in (q, k, v))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        q, k, v = (_rows16(x) for x in (q, k, v))   # kept for the backward as they are read
         out = _Cross.apply(q, k, v, lens, mask, scale)
     else:
         out = _forward(q, k, v, lens, mask, scale, False)[0]

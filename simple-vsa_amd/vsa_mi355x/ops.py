@@ -9,7 +9,9 @@ model keeps the op inside its graph:
 * ``vsa_mi355x::vsa_fwd`` / ``vsa_mi355x::vsa_bwd`` -- the full op
   (``torch_vsa`` / ``triton_vsa``, torch_impl.py:49-113);
 * ``vsa_mi355x::sparse_fwd`` / ``vsa_mi355x::sparse_bwd`` -- the explicit-route
-  fine branch (``triton_sparse_attention``, triton_impl.py:1626-1652).
+  fine branch (``triton_sparse_attention``, triton_impl.py:1626-1652);
+* ``vsa_mi355x::rotary`` -- rotary positions (its own gradient);
+* ``vsa_mi355x::cross_fwd`` / ``vsa_mi355x::cross_bwd`` -- cross attention.
 
 ``mi355x_vsa`` and ``mi355x_sparse_attention`` below keep the reference
 signatures and validation and give the same values as the eager functions of
@@ -26,7 +28,9 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
+from . import cross as X
 from . import mi355x as M
+from . import rotary as R
 
 
 def _empty(like: Tensor, dtype=None) -> Tensor:
@@ -209,3 +213,116 @@ def mi355x_sparse_attention(q: Tensor, k: Tensor, v: Tensor, selected: Tensor,
     vbs = M._i32(variable_block_sizes, q.device)
     save = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     return sparse_fwd(q, k, v, sel, vbs, be, float(scale), save)[0]
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions
+# ---------------------------------------------------------------------------
+
+@torch.library.custom_op("vsa_mi355x::rotary", mutates_args=(), device_types="cuda")
+def rotary(q: Tensor, k: Optional[Tensor], cos: Tensor, sin: Tensor, positions: Optional[Tensor],
+           interleaved: bool, inverse: bool) -> Tuple[Tensor, Tensor]:
+    """(q turned, k turned); the second is an empty placeholder without k."""
+    q, k = R._rotate(q, k, cos, sin, positions, interleaved, inverse)
+    return q, (k if k is not None else _empty(q))
+
+
+@rotary.register_fake
+def _(q, k, cos, sin, positions, interleaved, inverse):
+    return R.empty_in_order(q), (R.empty_in_order(k) if k is not None else _empty(q))
+
+
+def _rotary_setup(ctx, inputs, output):
+    q, k, cos, sin, positions, interleaved, inverse = inputs
+    ctx.save_for_backward(cos, sin, positions)
+    ctx.options = k is not None, interleaved, inverse
+
+
+def _rotary_backward(ctx, gq, gk):
+    cos, sin, positions = ctx.saved_tensors
+    has_k, interleaved, inverse = ctx.options
+    gq, gk = rotary(gq, gk if has_k else None, cos, sin, positions, interleaved, not inverse)
+    return gq, (gk if has_k else None), None, None, None, None, None
+
+
+rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)
+
+
+def mi355x_rotary(q: Tensor, k: Optional[Tensor], cos: Tensor, sin: Tensor,
+                  positions: Optional[Tensor] = None, *, interleaved: bool = False,
+                  inverse: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+    """``vsa_mi355x.mi355x_rotary`` through the custom op: the same checks, values
+    and gradients."""
+    R._check_rotary(q, k, cos, sin, positions)
+    if q.numel() == 0 or (k is not None and k.numel() == 0):
+        return R.mi355x_rotary(q, k, cos, sin, positions, interleaved=interleaved, inverse=inverse)
+    positions = None if positions is None else positions.contiguous()
+    q, turned = rotary(q, k, cos.contiguous(), sin.contiguous(), positions, bool(interleaved),
+                       bool(inverse))
+    return q, (turned if k is not None else None)
+
+
+# ---------------------------------------------------------------------------
+# Cross attention
+# ---------------------------------------------------------------------------
+
+@torch.library.custom_op("vsa_mi355x::cross_fwd", mutates_args=(), device_types="cuda")
+def cross_fwd(q: Tensor, k: Tensor, v: Tensor, lens: Optional[Tensor], mask: Optional[Tensor],
+              scale: float, save: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """(out, lo, lse); the last two are empty placeholders without ``save`` (lo also
+    in fp32)."""
+    out, lo, lse = X._forward(q, k, v, lens, mask, scale, save)
+    return (out, lo if lo is not None else _empty(q),
+            lse if lse is not None else _empty(q, torch.float32))
+
+
+@cross_fwd.register_fake
+def _(q, k, v, lens, mask, scale, save):
+    lo = q.new_empty(q.shape) if save and q.dtype != torch.float32 else _empty(q)
+    lse = (q.new_empty(q.shape[:3], dtype=torch.float32) if save else _empty(q, torch.float32))
+    return R.empty_in_order(q), lo, lse
+
+
+@torch.library.custom_op("vsa_mi355x::cross_bwd", mutates_args=(), device_types="cuda")
+def cross_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, lens: Optional[Tensor],
+              mask: Optional[Tensor], out: Tensor, lo: Tensor, lse: Tensor, scale: float
+              ) -> Tuple[Tensor, Tensor, Tensor]:
+    return X._backward(q, k, v, lens, mask, scale, out, lo if lo.numel() else None, lse, dout)
+
+
+@cross_bwd.register_fake
+def _(dout, q, k, v, lens, mask, out, lo, lse, scale):
+    return R.empty_in_order(q), R.empty_in_order(k), R.empty_in_order(v)
+
+
+def _cross_setup(ctx, inputs, output):
+    q, k, v, lens, mask, scale, _ = inputs
+    ctx.save_for_backward(q, k, v, lens, mask, *output)
+    ctx.scale = scale
+
+
+def _cross_backward(ctx, dout, *_):
+    q, k, v, lens, mask, out, lo, lse = ctx.saved_tensors
+    return (*cross_bwd(dout, q, k, v, lens, mask, out, lo, lse, ctx.scale), None, None, None, None)
+
+
+cross_fwd.register_autograd(_cross_backward, setup_context=_cross_setup)
+
+
+def mi355x_cross_attention(q: Tensor, k: Tensor, v: Tensor, kv_lens: Optional[Tensor] = None,
+                           key_mask: Optional[Tensor] = None, *,
+                           sm_scale: Optional[float] = None) -> Tensor:
+    """``vsa_mi355x.mi355x_cross_attention`` through the custom ops: the same checks,
+    values and gradients."""
+    X._check(q, k, v, kv_lens, key_mask, sm_scale)
+    d = q.shape[3]
+    if q.numel() == 0 or k.numel() == 0:
+        return X.mi355x_cross_attention(q, k, v, kv_lens, key_mask, sm_scale=sm_scale)
+    scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d)
+    lens = None if kv_lens is None else M._i32(kv_lens, q.device)
+    mask = None if key_mask is None else key_mask.contiguous()
+    if d % 8:
+        q, k, v = (torch.nn.functional.pad(x, (0, 8 - d % 8)) for x in (q, k, v))
+    save = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    out = cross_fwd(q, k, v, lens, mask, scale, save)[0]
+    return out[..., :d] if d % 8 else out

@@ -4,9 +4,12 @@
 // x2 cos a + x1 sin a); the gradient is the same rotation by -a.  Pairs are
 // channels (2i, 2i + 1) or (i, i + R/2) of the first R channels of a head.
 //
-// Both kernels are bound by memory: the rotation reads and writes q and k once
-// (the table adds 4 R bytes a token, shared by every head), the table is
-// written once.
+// Both are bound by memory.  The rotation reads and writes q and k once (the
+// table adds 4 R bytes a token and block of heads, from L2): 40 heads x 41k tokens
+// x 128 channels in 0.28 ms, 6.0 TB/s, where the best copy of this card reaches
+// 6.25.  The table is written once: 92160 positions x 64 pairs in 13 us, 3.6 TB/s
+// (runs of 8 / 16 / 32 positions: 17.9 / 14.1 / 13.0 us, and 9.6 / 8.3 / 9.5 for
+// 32760 x 64).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -89,7 +92,7 @@ struct RotaryArgs {
   int64_t pos_batch;    // elements between two samples' positions
   int64_t rows;         // of the table
   int64_t tokens;
-  int32_t pos64, heads_q, heads, dim, pairs, units, turns, per_block, head_blocks;
+  int32_t pos64, heads_q, heads, dim, pairs, units, turns, per_block, head_blocks, heads_fastest;
   float sign;
 };
 
@@ -113,29 +116,48 @@ __device__ __forceinline__ void st_piece(T* p, const Piece<T, V>& v) {
     *reinterpret_cast<Piece<T, V>*>(p) = v;
 }
 
-// A thread owns a unit of one token's channels, the same in every head, and walks
-// the heads of q and k with its cosines and sines in registers, so the table is
-// read once a token and not once a head.  A unit is V pairs in two pieces of V
-// channels, or with INTER V / 2 pairs in one piece (two pieces a thread left each
-// load instruction on every other 16 bytes: 24 heads x 16k tokens 61 -> TIME us),
-// or behind the turned channels a piece that is copied.  LOOSE: no alignment but
-// the element's (INTER with an odd start or end: elements one by one).
-template <typename T, int V, bool INTER, bool LOOSE>
+// A thread owns a unit of one token's channels, the same in up to per_block heads
+// of q and k, which it walks with its cosines and sines in registers.  A unit is
+//  * kInter: a piece of V channels, V / 2 pairs;
+//  * kSwap: a piece of V channels of which each is one of a pair; the other one's
+//    piece comes from the lane that has it (the units of a row divide a wave);
+//  * kTwo: V pairs, as a piece of either half (rows of other lengths; two loads of
+//    half a row each: 24 heads x 41k tokens of 64 channels 112 us, kSwap 85);
+//  * behind the turned channels, a piece that is copied.
+// LOOSE: no alignment but the element's (kInter with an odd start or end).
+enum RotaryMode { kTwo, kInter, kSwap };
+
+template <typename T, int V, int MODE, bool LOOSE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-  constexpr int P = INTER ? V / 2 : V;   // pairs of a unit
-  const int per = 256 / a.units;         // tokens of a workgroup
+  constexpr int P = MODE == kInter ? V / 2 : V;   // cosines of a unit
+  const int per = 256 / a.units;                  // tokens of a workgroup
   const int unit = threadIdx.x % a.units;
   if ((int)threadIdx.x >= per * a.units) return;
-  int64_t g = blockIdx.x;
-  const int hb = (int)(g % a.head_blocks);
-  g /= a.head_blocks;
+  // Head-major memory: the blocks of heads follow each other slowest, so that the
+  // workgroups at work read and write neighbouring rows of a few heads; token-major:
+  // fastest, so that they cover whole tokens (40 heads x 41k tokens, all heads in
+  // a workgroup / blocks of four or eight in that order: 309 -> 289 and 322 -> 291
+  // us, interleaved 321 -> 285 and 321 -> 273).
   const int64_t blocks = (a.tokens + per - 1) / per;
-  const int64_t b = g / blocks;
+  int64_t g = blockIdx.x;
+  int hb;
+  if (a.heads_fastest) {
+    hb = (int)(g % a.head_blocks);
+    g /= a.head_blocks;
+  }
   const int64_t t = g % blocks * per + threadIdx.x / a.units;
+  g /= blocks;
+  if (!a.heads_fastest) {
+    hb = (int)(g % a.head_blocks);
+    g /= a.head_blocks;
+  }
+  const int64_t b = g;
   if (t >= a.tokens) return;
   const bool turn = unit < a.turns;
   const int o1 = turn ? unit * V : 2 * a.pairs + (unit - a.turns) * V;
-  const int o2 = a.pairs + o1;           // the second piece, without INTER
+  const int o2 = a.pairs + o1;                    // kTwo: the second piece
+  const int half = a.pairs / V;                   // kSwap: units of half a row
+  const bool second = MODE == kSwap && unit >= half;
 
   float c[P], s[P];
 #pragma unroll
@@ -150,10 +172,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 #pragma unroll
       for (int e = 0; e < P; ++e) c[e] = s[e] = NAN;
     } else if (p >= 0) {
-      const float* cp = a.co + p * a.pairs + unit * P;
-      const float* sp = a.si + p * a.pairs + unit * P;
+      const int64_t at = p * a.pairs + (second ? unit - half : unit) * P;
+      const float sign = second ? -a.sign : a.sign;
 #pragma unroll
-      for (int e = 0; e < P; ++e) c[e] = cp[e], s[e] = sp[e] * a.sign;
+      for (int e = 0; e < P; ++e) c[e] = a.co[at + e], s[e] = a.si[at + e] * sign;
     }
   }
   auto load = [&](const T* x) {
@@ -181,7 +203,18 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
       const T* x = (const T*)a.x[w] + b * a.xs[w][0] + (hh - w * a.heads_q) * a.xs[w][1] +
                    t * a.xs[w][2];
       x1[u] = load(x + o1);
-      if (!INTER && turn) x2[u] = load(x + o2);
+      if (MODE == kTwo && turn) x2[u] = load(x + o2);
+    }
+    if constexpr (MODE == kSwap) {
+      typedef uint32_t Words __attribute__((ext_vector_type(V * sizeof(T) / 4)));
+      const int other = (int)(threadIdx.x & 63) + (turn ? second ? -half : half : 0);
+#pragma unroll
+      for (int u = 0; u < UR; ++u) {
+        Words w = __builtin_bit_cast(Words, x1[u]);
+#pragma unroll
+        for (int i = 0; i < (int)(V * sizeof(T) / 4); ++i) w[i] = __shfl(w[i], other, 64);
+        x2[u] = __builtin_bit_cast(Piece<T, V>, w);
+      }
     }
 #pragma unroll
     for (int u = 0; u < UR; ++u) {
@@ -191,40 +224,44 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
       if (turn) {
 #pragma unroll
         for (int e = 0; e < P; ++e) {
-          T& lo = INTER ? x1[u].e[2 * e] : x1[u].e[e];
-          T& hi = INTER ? x1[u].e[2 * e + 1] : x2[u].e[e];
+          T& lo = MODE == kInter ? x1[u].e[2 * e] : x1[u].e[e];
+          T& hi = MODE == kInter ? x1[u].e[2 * e + 1] : x2[u].e[e];
           const float p = Elem<T>::to_f(lo), q = Elem<T>::to_f(hi);
+          // (kSwap: the second of a pair has the sine's sign turned)
           lo = Elem<T>::from_f(p * c[e] - q * s[e]);
-          hi = Elem<T>::from_f(q * c[e] + p * s[e]);
+          if (MODE != kSwap) hi = Elem<T>::from_f(q * c[e] + p * s[e]);
         }
-        if (!INTER) store(y + o2, x2[u]);
+        if (MODE == kTwo) store(y + o2, x2[u]);
       }
       store(y + o1, x1[u]);
     }
   }
 }
 
-template <typename T, int V, bool INTER, bool LOOSE = false>
+template <typename T, int V, int MODE, bool LOOSE = false>
 static int launch_rotary(const RotaryArgs& a, int64_t batch, hipStream_t s) {
   const int per = 256 / a.units;
   const int64_t grid = (a.tokens + per - 1) / per * batch * a.head_blocks;
   if (grid > (1LL << 31) - 1) return VSA_ERR_SHAPE;
-  hipLaunchKernelGGL((rotary_kernel<T, V, INTER, LOOSE>), dim3((unsigned)grid), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((rotary_kernel<T, V, MODE, LOOSE>), dim3((unsigned)grid), dim3(256), 0, s, a);
   return vsa_check_launch();
 }
 
 // v: channels of a piece that every start and length allows
 template <typename T>
-static int rotary_of(const RotaryArgs& a, int64_t batch, int v, bool inter, hipStream_t s) {
+static int rotary_of(const RotaryArgs& a, int64_t batch, int v, int mode, hipStream_t s) {
+  constexpr int W = 16 / sizeof(T);
+  if (mode == kSwap) return launch_rotary<T, W, kSwap>(a, batch, s);   // (v is W)
+  const bool inter = mode == kInter;
   if constexpr (sizeof(T) == 2) {
     if (v == 8)
-      return inter ? launch_rotary<T, 8, true>(a, batch, s) : launch_rotary<T, 8, false>(a, batch, s);
+      return inter ? launch_rotary<T, 8, kInter>(a, batch, s) : launch_rotary<T, 8, kTwo>(a, batch, s);
   }
   if (v == 4)
-    return inter ? launch_rotary<T, 4, true>(a, batch, s) : launch_rotary<T, 4, false>(a, batch, s);
+    return inter ? launch_rotary<T, 4, kInter>(a, batch, s) : launch_rotary<T, 4, kTwo>(a, batch, s);
   if (v == 2)
-    return inter ? launch_rotary<T, 2, true>(a, batch, s) : launch_rotary<T, 2, false>(a, batch, s);
-  return inter ? launch_rotary<T, 2, true, true>(a, batch, s) : launch_rotary<T, 1, false>(a, batch, s);
+    return inter ? launch_rotary<T, 2, kInter>(a, batch, s) : launch_rotary<T, 2, kTwo>(a, batch, s);
+  return inter ? launch_rotary<T, 2, kInter, true>(a, batch, s) : launch_rotary<T, 1, kTwo>(a, batch, s);
 }
 
 }  // namespace vsa
@@ -323,16 +360,16 @@ extern "C" int vsa_rotary(const vsa_rotary_op* op, void* stream) {
   a.heads_q = op->q_heads, a.heads = op->q_heads + op->k_heads;
   a.dim = op->head_dim, a.pairs = op->channels / 2;
   const int unit = inter && v == 1 ? 2 : v;
-  a.turns = (inter ? op->channels : a.pairs) / unit;
-  a.units = a.turns + (op->head_dim - op->channels + unit - 1) / unit;
+  const int rest = (op->head_dim - op->channels + unit - 1) / unit;
+  int mode = inter ? kInter : kTwo;
+  if (!inter && v * es == 16 && 64 % (op->channels / v + rest) == 0) mode = kSwap;
+  a.turns = (mode == kTwo ? a.pairs : op->channels) / unit;
+  a.units = a.turns + rest;
   a.sign = op->inverse ? -1.f : 1.f;
-  const int per = 256 / a.units;
-  const int64_t blocks = (a.tokens + per - 1) / per * op->batch;
-  // a workgroup walks every head where the tokens fill the chip, else a part
-  int64_t split = blocks >= 1024 ? 1 : (1024 + blocks - 1) / blocks;
-  if (split > (a.heads + 3) / 4) split = (a.heads + 3) / 4;
-  a.per_block = (int)((a.heads + split - 1) / split);
+  // token-major memory, by q's strides
+  a.heads_fastest = op->q_heads > 1 && op->tokens > 1 && a.xs[0][1] < a.xs[0][2];
+  a.per_block = a.heads_fastest ? 8 : 4;
   a.head_blocks = (a.heads + a.per_block - 1) / a.per_block;
   hipStream_t s = (hipStream_t)stream;
-  VSA_DISPATCH_ALL(op->dtype, T, return rotary_of<T>(a, op->batch, v, inter, s));
+  VSA_DISPATCH_ALL(op->dtype, T, return rotary_of<T>(a, op->batch, v, mode, s));
 }

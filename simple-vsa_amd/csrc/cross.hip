@@ -29,7 +29,7 @@ int check(const vsa_cross* c) {
   if (c->batch <= 0 || c->batch > 65535 || c->heads <= 0 || c->kv_heads <= 0 ||
       c->heads % c->kv_heads || c->heads > 65535 || c->head_dim <= 0 || c->head_dim > 256 ||
       c->head_dim % 8 || c->sq <= 0 || c->skv <= 0 || c->skv > (1LL << 31) - 256 ||
-      c->sq > ((1LL << 31) - 256) / (c->heads / c->kv_heads) || !(c->scale - c->scale == 0.f) ||
+      c->sq > ((1LL << 31) - 256) / (c->heads / c->kv_heads) || !(fabsf(c->scale) <= 0x1p127f) ||
       (c->key_mask && c->mask_stride < 0) || c->q_stride[2] < c->head_dim ||
       c->k_stride[2] < c->head_dim || c->v_stride[2] < c->head_dim)
     return VSA_ERR_SHAPE;

@@ -27,6 +27,7 @@ from .rotary import empty_in_order, strides
 
 MAX_HEAD_DIM = 256
 MAX_TOKENS = (1 << 31) - 256
+MAX_SCALE = 2.0 ** 127   # times log2(e) it stays finite in fp32
 
 
 def _rows16(x: Tensor) -> Tensor:
@@ -58,13 +59,21 @@ def _pack(q, k, v, lens, mask, scale) -> bytes:
         _lib.DTYPE_CODES[q.dtype], scale)
 
 
+def _lens(kv_lens: Optional[Tensor], skv: int, device) -> Optional[Tensor]:
+    """kv_lens as the kernels read it; 64-bit ones are clamped before they lose bits."""
+    if kv_lens is None:
+        return None
+    return _i32(kv_lens.clamp(0, skv) if kv_lens.dtype is torch.int64 else kv_lens, device)
+
+
 def _three(x: Tensor) -> bytes:
     return _lib.STRIDES.pack(*_strides(x))
 
 
 @functools.lru_cache(maxsize=256)
-def _sizes(b, h, hk, sq, skv, d, lens, masked, dtype):
-    """Bytes of (forward scratch, backward scratch)."""
+def _sizes(b, h, hk, sq, skv, d, lens, masked, dtype, device):
+    """Bytes of (forward scratch, backward scratch) on ``device``, the current one
+    (the splits follow its number of CUs)."""
     # a pointer's presence is all that is read
     c = _lib.CROSS.pack(256, 256, 256, 256 if lens else 0, 256 if masked else 0, *(0, 0, 256) * 3, 0, sq, skv, b, h,
                         hk, d, dtype, 1.0)
@@ -77,7 +86,8 @@ def _sizes(b, h, hk, sq, skv, d, lens, masked, dtype):
 def _scratch(q, k, lens, mask, which: int) -> Optional[Tensor]:
     b, h, sq, d = q.shape
     return _workspace(_sizes(b, h, k.shape[1], sq, k.shape[2], d, lens is not None,
-                             mask is not None, _lib.DTYPE_CODES[q.dtype])[which], q.device)
+                             mask is not None, _lib.DTYPE_CODES[q.dtype], q.device.index)[which],
+                      q.device)
 
 
 def _forward(q, k, v, lens, mask, scale, keep):
@@ -156,8 +166,8 @@ def _check(q, k, v, kv_lens, key_mask, sm_scale) -> None:
             raise ValueError("key_mask must have shape [batch, kv seq_len]")
         if key_mask.dtype != torch.bool:
             raise ValueError("key_mask must be bool (True: the key is attended to)")
-    if sm_scale is not None and not math.isfinite(sm_scale):
-        raise ValueError("sm_scale must be finite")
+    if sm_scale is not None and not abs(sm_scale) <= MAX_SCALE:
+        raise ValueError("sm_scale must be finite, and lie within 2^127")
     if b > 65535 or h > 65535 or k.shape[2] > MAX_TOKENS or \
             (h and sq > MAX_TOKENS // (h // k.shape[1])):
         raise ValueError("the MI355X kernels support at most 65535 samples and heads, and fewer "
@@ -191,7 +201,7 @@ def mi355x_cross_attention(q: Tensor, k: Tensor, v: Tensor, kv_lens: Optional[Te
         rest = sum(x[..., :0].sum() for x in (q, k, v))
         return torch.zeros(q.shape, dtype=q.dtype, device=q.device) + rest
     scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d)
-    lens = None if kv_lens is None else _i32(kv_lens, q.device)
+    lens = _lens(kv_lens, k.shape[2], q.device)
     mask = key_mask
     if mask is not None and mask.stride(1) != 1 and mask.shape[1] > 1:
         mask = mask.contiguous()

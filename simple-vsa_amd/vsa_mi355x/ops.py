@@ -319,7 +319,7 @@ def mi355x_cross_attention(q: Tensor, k: Tensor, v: Tensor, kv_lens: Optional[Te
     if q.numel() == 0 or k.numel() == 0:
         return X.mi355x_cross_attention(q, k, v, kv_lens, key_mask, sm_scale=sm_scale)
     scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d)
-    lens = None if kv_lens is None else M._i32(kv_lens, q.device)
+    lens = X._lens(kv_lens, k.shape[2], q.device)
     mask = None if key_mask is None else key_mask.contiguous()
     if d % 8:
         q, k, v = (torch.nn.functional.pad(x, (0, 8 - d % 8)) for x in (q, k, v))

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -85,7 +86,8 @@ def build_rotary_table(dit_seq_shape: Tuple[int, int, int], axis_channels: Tuple
     those that turn once or less, a ramp between, and multiplies cos and sin by
     ``0.1 ln(factor) + 1``.  Angles are made in 64 bits."""
     axes, tokens, pairs = _axes(
-        _three(dit_seq_shape, "dit_seq_shape", int), _three(axis_channels, "axis_channels", int),
+        _three(dit_seq_shape, "dit_seq_shape", operator.index),
+        _three(axis_channels, "axis_channels", operator.index),
         float(theta), _three(start, "start"), _three(factor, "factor"), method,
         None if original_shape is None else _three(original_shape, "original_shape"))
     device = torch.device(device)

@@ -123,3 +123,25 @@ def test_workspaces_are_bounded():
         c.sq, c.skv, c.batch, c.heads, c.kv_heads, c.head_dim, c.scale = sq, skv, b, h, h, d, 1.0
         assert lib.vsa_cross_sizes(ctypes.addressof(c), at, at + 8) == 0
         assert n[0] <= 1 << 28 and n[1] <= 1 << 30, (n[0], n[1])
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3e38, -3e38])
+def test_scales_that_fp32_cannot_hold_in_base_two_are_refused(scale):
+    with pytest.raises(ValueError, match="finite"):
+        mi355x_cross_attention(**_args(sm_scale=scale))
+    c = Cross()
+    c.q = c.k = c.v = 256
+    c.q_stride[:] = c.k_stride[:] = c.v_stride[:] = [64, 64, 64]
+    c.sq, c.skv, c.batch, c.heads, c.kv_heads, c.head_dim = 4, 6, 2, 4, 2, 64
+    n = (ctypes.c_int64 * 2)()
+    at = ctypes.addressof(n)
+    for c.scale, rc in ((scale, -2), (2.0 ** 127, 0), (-2.0 ** 127, 0)):
+        assert _lib.load().vsa_cross_sizes(ctypes.addressof(c), at, at + 8) == rc
+
+
+def test_lengths_of_64_bits_are_clamped_before_they_lose_bits():
+    from vsa_mi355x.cross import _lens
+    lens = torch.tensor([(1 << 32) + 3, -(1 << 32) + 3, 1 << 31, 5, -1])
+    assert _lens(lens, 7, lens.device).tolist() == [7, 0, 7, 5, 0]
+    assert _lens(lens, 7, lens.device).dtype == torch.int32
+    assert _lens(None, 7, lens.device) is None

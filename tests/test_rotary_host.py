@@ -30,6 +30,12 @@ def test_table_refusals(args, kw, text):
         build_rotary_table(*args, **kw)
 
 
+@pytest.mark.parametrize("args", [((2, 2.5, 2), (4, 4, 4)), ((2, 2, 2), (4, 4.0, 4))])
+def test_table_sizes_are_integers(args):
+    with pytest.raises(TypeError):
+        build_rotary_table(*args)
+
+
 def _args(**kw):
     a = dict(q=torch.zeros(2, 3, 5, 16), k=torch.zeros(2, 1, 5, 16), cos=torch.zeros(5, 8),
              sin=torch.zeros(5, 8), positions=None)

@@ -344,6 +344,17 @@ __device__ __forceinline__ int tile_of(const CrossArgs& a) {
 
 typedef const __attribute__((address_space(4))) uint32_t* const_words;
 
+// Whether a sample's first n keys hold a single valid one.  Its weight is 1 whatever
+// the scores and dS is 0, where P (dP - delta) would leave the rounding of two sums
+// over the channels: gradients of q and k that are nothing but noise.
+__device__ __forceinline__ bool single_key(const CrossArgs& a, int b, int n) {
+  if (!a.words) return n == 1;
+  const const_words words = (const_words)(uintptr_t)(a.words + (int64_t)b * a.nwords);
+  int count = 0;
+  for (int x = 0; x < (n + 31) / 32 && count < 2; ++x) count += __builtin_popcount(words[x]);
+  return count == 1;
+}
+
 // The chunks of KC keys of one sample that hold a valid key, in order.  The
 // words are read through the constant address space: scalar loads, which the
 // direct copies' vmcnt waits never include.

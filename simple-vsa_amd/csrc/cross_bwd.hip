@@ -68,6 +68,7 @@ void cross_dq_kernel(CrossArgs a) {
   const int per_split = (chunks + a.splits - 1) / a.splits;
   KeyWalk<KC> walk;
   walk.init(a, b, split * per_split, per_split);
+  const float some = single_key(a, b, walk.n) ? 0.f : 1.f;
   auto copy = [&](int stage) __attribute__((always_inline)) {
     const int left = walk.n - walk.j * KC;
     const auto ks = kcopy.rows(kbase + (int64_t)walk.j * KC * a.k.s, left);
@@ -171,12 +172,12 @@ void cross_dq_kernel(CrossArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         ds[x][i] = fast_exp2(fmaf(s[x][i], a.c2, -lse)) * (dp[x][i] - delta);
-    if (!whole) {   // (a masked key's P may be infinite)
+    if (!whole) {   // (a masked key's P may be infinite; a single key's chunk is never whole)
       keep_branch();
 #pragma unroll
       for (int x = 0; x < C::NSM; ++x)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ds[x][i] = acc_valid(w[x], i) ? ds[x][i] : 0.f;
+        for (int i = 0; i < 16; ++i) ds[x][i] = acc_valid(w[x], i) ? ds[x][i] * some : 0.f;
     }
 #pragma unroll
     for (int kk = 0; kk < 2 * C::NSM; ++kk) {
@@ -253,8 +254,13 @@ struct CrossDkvCfg {
   static constexpr int wait(int items) { return items * PER < 63 ? items * PER : 63; }
   static constexpr int NA = 2 * (D / 16);                // Q and dO rows
   static constexpr int NC = 4 * (DA / 32);               // dO and Q columns
-  static constexpr int AHEAD = D > 128 ? 4 : KT > 1 ? 6 : 12;
   static constexpr int NV = 16 * KT;                     // P values of a lane per item
+  // Up to 64 keys (128 at head dim 64) the pass reads Q and dO for longer than it
+  // multiplies, and dK takes what rounding dS leaves over as well: 16k queries on 32
+  // keys 42 -> 45 us at head dim 128, 29 -> 33 on 64 at head dim 64, dK off 1.7e-3 of
+  // its norm instead of 2.4e-3.  For more keys it stays out (512: 241 -> 288 us).
+  static constexpr bool BOTH = PIPE && NW <= 2;
+  static constexpr int AHEAD = D > 128 || (KT > 1 && BOTH) ? 4 : KT > 1 ? 6 : 12;
 };
 
 template <typename T, int D, int NW>
@@ -496,9 +502,16 @@ void cross_dkv_kernel(CrossArgs a) {
         value(u);
         __builtin_amdgcn_sched_barrier(0);
       }
-      V8 bp[KT][2], bs[KT][2];
+      V8 bp[KT][2], bs[KT][2], bl[KT][2];
+      auto pack = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-      for (int t = 0; t < KT; ++t) bp[t][0] = pack_op<T>(pv[t]), bs[t][0] = pack_op<T>(ds[t]);
+        for (int t = 0; t < KT; ++t) {
+          bp[t][j] = pack_op<T>(pv[t] + 8 * j);
+          if constexpr (C::BOTH) pack_both<T>(ds[t] + 8 * j, bs[t][j], bl[t][j]);
+          else bs[t][j] = pack_op<T>(ds[t] + 8 * j);
+        }
+      };
+      pack(0);
 #pragma unroll
       for (int y = 0; y < NC; ++y) {
         issue(NA + y + L);
@@ -507,16 +520,13 @@ void cross_dkv_kernel(CrossArgs a) {
         for (int t = 0; t < KT; ++t) {
           if (y & 1) dk[mt][t] = M::mul(op[NA + y], bs[t][j], dk[mt][t]);
           else dv[mt][t] = M::mul(op[NA + y], bp[t][j], dv[mt][t]);
+          if (C::BOTH && (y & 1)) dk[mt][t] = M::mul(op[NA + y], bl[t][j], dk[mt][t]);
         }
 #pragma unroll
         for (int p = 0; p < C::PER; ++p)
           if (NC / 2 + p * (NC / 2) / C::PER == y) piece(cp, SP, p);
         if (y < NC / 2) value(NA + y);
-        if (y == NC / 2 - 1) {
-#pragma unroll
-          for (int t = 0; t < KT; ++t)
-            bp[t][1] = pack_op<T>(pv[t] + 8), bs[t][1] = pack_op<T>(ds[t] + 8);
-        }
+        if (y == NC / 2 - 1) pack(1);
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
@@ -542,6 +552,7 @@ void cross_dkv_kernel(CrossArgs a) {
   }
 
   // keys that are not valid get zeros
+  const float dk_scale = single_key(a, b, __builtin_amdgcn_readfirstlane(n)) ? 0.f : a.scale;
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
     const int key = key0 + 32 * t;
@@ -551,7 +562,7 @@ void cross_dkv_kernel(CrossArgs a) {
     float wk[2][8], wv[2][8];
 #pragma unroll
     for (int mt = 0; mt < DA / 32; ++mt) {
-      swap_rows16(dk[mt][t], a.scale, wk);
+      swap_rows16(dk[mt][t], dk_scale, wk);
       swap_rows16(dv[mt][t], 1.f, wv);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {

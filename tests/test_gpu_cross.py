@@ -396,3 +396,51 @@ def test_a_blocks_attention_together():
         again = mi355x_vsa_tiled(qr.transpose(1, 2), kr.transpose(1, 2), leaves[2], shape, nb, tile,
                                  token_major=True)
     assert torch.equal(a, again)
+
+
+@pytest.mark.parametrize("how", ["one", "lens", "mask", "both"])
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 40), ("fp32", 64), ("bf16", 256)])
+def test_a_single_valid_key_has_no_gradient_of_q_and_k(dtype, d, how):
+    """Its weight is 1 whatever the scores: the output is its value, dv the sum of the
+    outputs' gradients, dq and dk exactly zero.  The other sample is an ordinary one."""
+    from vsa_mi355x import mi355x_cross_attention
+    n = 1 if how == "one" else 200
+    host = _inputs(dtype, 2, 4, 2, 37, n, d, seed=41)
+    lens = mask = None
+    at = 0
+    if how in ("lens", "both"):
+        lens = torch.tensor([n if how == "both" else 1, 150], dtype=torch.int32)
+    if how in ("mask", "both"):
+        at = 170
+        mask = torch.zeros(2, n, dtype=torch.bool)
+        mask[0, at] = True
+        mask[1, ::3] = True
+    lens, mask = (None if x is None else x.to(DEV) for x in (lens, mask))
+    leaves = [x.to(DEV).requires_grad_() for x in host[:3]]
+    out = mi355x_cross_attention(*leaves, lens, mask)
+    grads = torch.autograd.grad(out, leaves, host[3].to(DEV))
+    ref, tol = reference(*(x.to(DEV) for x in host), lens, mask)
+    _check(NAMES, [out, *grads], ref, tol)
+    if dtype != "fp32":   # (there the weight and its inverse round: within the bound above)
+        one = leaves[2][0, :, at:at + 1].repeat_interleave(2, 0)
+        assert torch.equal(out[0], one.expand_as(out[0]))
+    for x in grads[:2]:
+        assert not x[0].any() and (how == "one" or x[1].any())
+
+
+@pytest.mark.parametrize("n,d", [(3, 40), (60, 128), (100, 64)])
+def test_few_keys_take_no_more_rounding_than_their_results(n, d):
+    """dk of a prompt of a few keys is off by little more than its own rounding: dS
+    enters the product with its rounding's rest."""
+    from vsa_mi355x import mi355x_cross_attention
+    host = _inputs("bf16", 3, 8, 4, 691, n, d, seed=43)
+    leaves = [x.to(DEV).requires_grad_() for x in host[:3]]
+    grads = torch.autograd.grad(mi355x_cross_attention(*leaves), leaves, host[3].to(DEV))
+    ref, _ = reference(*(x.to(DEV) for x in host))
+    for name, x, y in zip(NAMES[1:], grads, ref[1:]):
+        # the rest is itself rounded, 2^-16 of dS, and the fp32 sums are off by less:
+        # 1/256 of the result's own rounding, which 1.15 leaves room for (dS rounded
+        # once would make it sqrt(2)); P enters dv rounded once
+        if name != "dv":
+            own = (y.to(torch.bfloat16).double() - y).norm()
+            assert (x.double() - y).norm() <= 1.15 * own, name

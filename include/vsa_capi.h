@@ -513,9 +513,10 @@ int vsa_rotary(const vsa_rotary_op* op, void* stream);
  *
  * lse (fp32 [batch, heads, sq], NULL: not wanted) is the base-2 log-sum-exp the
  * backward needs, -inf without a valid key; lo ([batch, heads, sq, head_dim],
- * dense, 16-byte aligned; NULL: not wanted) is what rounding out to bf16 / fp16
- * left over, which a backward with it takes its row sums of dout * out from
- * (without it dq loses up to two bits; unused in fp32).  dk and dv are written for every
+ * dense, a byte each, 8-byte aligned; NULL: not wanted) is what rounding out to
+ * bf16 / fp16 left over (1/254 of out's unit in the last place, 128 for nothing),
+ * which a backward with it takes its row sums of dout * out from (without it dq
+ * loses up to two bits; unused in fp32).  dk and dv are written for every
  * key (zeros where it is not valid) and summed over the heads that share a key
  * head, in a fixed order.  Scratch sizes come from vsa_cross_sizes, from
  * the sizes and from which pointers are NULL (256-byte aligned; 0: NULL will do).

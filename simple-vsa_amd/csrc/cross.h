@@ -13,6 +13,8 @@
 // row) takes part in a product.
 #pragma once
 
+#include <type_traits>
+
 #include "vsa_device.h"
 #include "vsa_launch.h"
 
@@ -315,7 +317,7 @@ struct Rows {          // a [batch, head, token] view
 struct CrossArgs {
   Rows q, k, v, o, dout;
   void *out, *dq, *dk, *dv;
-  void *lo;                    // what rounding the output left over, [batch, heads, sq, dim], or null
+  uint8_t* lo;                 // what rounding the output left over, [batch, heads, sq, dim], or null
   int64_t out_s[3], dq_s[3], dk_s[3], dv_s[3];
   float *lse, *delta;          // [batch, heads, sq]
   float *part_a, *part_b;      // fp32 partial results of the splits
@@ -423,22 +425,54 @@ __device__ __forceinline__ void st8(T* p, const float (&v)[8]) {
   }
 }
 
+// What rounding an output value o to 16 bits left over, as a byte: in units of
+// 1/254 of o's unit in the last place, 128 for nothing.  kLeast keeps the unit of
+// fp16's subnormals, and bf16's inverse finite.
+template <typename T>
+struct RestOf {
+  static constexpr bool kHalf = std::is_same<T, _Float16>::value;
+  static constexpr uint32_t kLeast = (127u - (kHalf ? 14u : 100u)) << 23;
+  static constexpr float kUnits = 127.f * (float)(1 << (kHalf ? 11 : 8));
+  static __device__ __forceinline__ uint32_t power(float o) {   // 2^exponent of o, as bits
+    return max(__float_as_uint(o) & 0x7f800000u, kLeast);
+  }
+};
+
 // Eight channels of the output, and what rounding them to T left over: delta is
 // sum dO O, and where the weights are spread over many keys dS = P (dP - delta)
 // is so much smaller than dP that the rounding of O shows in dQ (bf16, 4000
 // keys: 6.6e-3 of its norm, 1e-5 with the rest; the roundings that stay, of dS
-// and of dQ, make 2.4e-3).
+// and of dQ, make 2.4e-3).  A byte holds it to 2^-8 of itself, as 16 bits would.
 template <typename T>
-__device__ __forceinline__ void st8_out(T* out, T* lo, const float (&v)[8]) {
+__device__ __forceinline__ void st8_out(T* out, uint8_t* lo, const float (&v)[8]) {
   st8<T>(out, v);
   if constexpr (sizeof(T) == 2) {
     if (lo) {
-      float rest[8];
+      typedef RestOf<T> R;
+      uint32_t w[2] = {0, 0};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) rest[e] = v[e] - round_t<T>(v[e]);
-      st8<T>(lo, rest);
+      for (int e = 0; e < 8; ++e) {
+        const float o = round_t<T>(v[e]);
+        const float per = __uint_as_float(0x7f000000u - R::power(o)) * R::kUnits;
+        w[e >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(rintf(fmaf(v[e] - o, per, 128.f)), e & 3, w[e >> 2]);
+      }
+      *reinterpret_cast<u32x2*>(lo) = u32x2{w[0], w[1]};
     }
   }
+}
+
+// The sum of eight channels' g o with the rests of o.
+template <typename T>
+__device__ __forceinline__ float dot_rest(typename Mma<T>::V8 g, typename Mma<T>::V8 o, u32x2 rest,
+                                          float sum) {
+  typedef RestOf<T> R;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float n = (float)((rest[e >> 2] >> (8 * (e & 3))) & 255u), x = (float)o[e];
+    const float units = fmaf(n, 1.f / R::kUnits, -128.f / R::kUnits);
+    sum = fmaf((float)g[e], fmaf(units, __uint_as_float(R::power(x)), x), sum);
+  }
+  return sum;
 }
 
 }  // namespace vsa

@@ -94,11 +94,11 @@ extern "C" int vsa_cross_fwd(const vsa_cross* c, void* out, const int64_t* out_s
   if (!out || !out_stride) return VSA_ERR_NULL;
   if (!scratch && (c->key_mask || cross_fwd_parts(c))) return VSA_ERR_NULL;
   if (!rows_ok(out, out_stride, c->dtype == VSA_F32 ? 4 : 2) || !vsa_aligned<4>(lse) ||
-      !vsa_aligned<16>(lo) || !vsa_aligned<256>(scratch))
+      !vsa_aligned<8>(lo) || !vsa_aligned<256>(scratch))
     return VSA_ERR_ALIGN;
   CrossArgs a = args(c);
   a.out = out;
-  a.lo = lo;
+  a.lo = (uint8_t*)lo;
   for (int x = 0; x < 3; ++x) a.out_s[x] = out_stride[x];
   a.lse = lse;
   if (a.c2 < 0) {   // the running max wants a scale that keeps the order
@@ -122,7 +122,7 @@ extern "C" int vsa_cross_bwd(const vsa_cross* c, const void* out, const int64_t*
   const int es = c->dtype == VSA_F32 ? 4 : 2;
   if (!rows_ok(out, out_stride, es) || !rows_ok(dout, dout_stride, es) ||
       !rows_ok(dq, dq_stride, es) || !rows_ok(dk, dk_stride, es) || !rows_ok(dv, dv_stride, es) ||
-      !vsa_aligned<16>(lo) || !vsa_aligned<4>(lse) || !vsa_aligned<256>(scratch))
+      !vsa_aligned<8>(lo) || !vsa_aligned<4>(lse) || !vsa_aligned<256>(scratch))
     return VSA_ERR_ALIGN;
   CrossArgs a = args(c);
   a.o = {out, out_stride[0], out_stride[1], out_stride[2]};
@@ -130,7 +130,7 @@ extern "C" int vsa_cross_bwd(const vsa_cross* c, const void* out, const int64_t*
   a.dq = dq, a.dk = dk, a.dv = dv;
   for (int x = 0; x < 3; ++x)
     a.dq_s[x] = dq_stride[x], a.dk_s[x] = dk_stride[x], a.dv_s[x] = dv_stride[x];
-  a.lo = const_cast<void*>(lo);
+  a.lo = (uint8_t*)const_cast<void*>(lo);
   a.lse = const_cast<float*>(lse);
   char* at = (char*)scratch;
   if ((rc = prepare(c, a, at, (hipStream_t)stream))) return rc;

@@ -104,7 +104,10 @@ void cross_dq_kernel(CrossArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     };
     const bool rest = sizeof(T) == 2 && a.lo;
-    const T* lrow = (const T*)a.lo + stat * a.dim;
+    const uint8_t* lrow = a.lo + stat * a.dim;
+    auto rests = [&](int d) __attribute__((always_inline)) {
+      return *reinterpret_cast<const u32x2*>(lrow + d);
+    };
     auto dot = [&](V8 g, V8 o) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) delta = fmaf((float)g[e], (float)o[e], delta);
@@ -115,21 +118,39 @@ void cross_dq_kernel(CrossArgs a) {
       for (int ks = 0; ks < D / 16; ++ks) {
         const int d = 16 * ks + 8 * h;
         if (d < a.dim) {
-          dot(gf[ks], ld8<T>(orow + d));
-          if (rest) dot(gf[ks], ld8<T>(lrow + d));
+          const V8 o = ld8<T>(orow + d);
+          if constexpr (sizeof(T) == 2) {
+            if (rest) {
+              delta = dot_rest<T>(gf[ks], o, rests(d), delta);
+              continue;
+            }
+          }
+          dot(gf[ks], o);
         }
       }
       load(qf, qrow);
     } else {
-      V8 of[D / 16], lf[D / 16];
+      V8 of[D / 16];
+      u32x2 lf[D / 16];
       load(gf, grow);
       load(of, orow);
-      if (rest) load(lf, lrow);
+      if (rest) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+          lf[ks] = 16 * ks + 8 * h < a.dim ? rests(16 * ks + 8 * h) : u32x2{0, 0};
+        __builtin_amdgcn_sched_barrier(0);
+      }
       load(qf, qrow);
+      // (channels past the head dim: g is 0, and o and its rest are finite)
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
+        if constexpr (sizeof(T) == 2) {
+          if (rest) {
+            delta = dot_rest<T>(gf[ks], of[ks], lf[ks], delta);
+            continue;
+          }
+        }
         dot(gf[ks], of[ks]);
-        if (rest) dot(gf[ks], lf[ks]);
       }
     }
     delta = pair_sum32(delta);

@@ -205,7 +205,7 @@ void cross_fwd_kernel(CrossArgs a) {
   }
   T* orow = (T*)a.out + b * a.out_s[0] + head * a.out_s[1] + sq_i * a.out_s[2];
   const int64_t stat = ((int64_t)b * a.heads + head) * a.sq + sq_i;
-  T* lrow = a.lo ? (T*)a.lo + stat * a.dim : nullptr;
+  uint8_t* lrow = a.lo ? a.lo + stat * a.dim : nullptr;
 #pragma unroll
   for (int mt = 0; mt < D / 32; ++mt) {
     swap_rows16(oacc[mt], inv, w8);
@@ -431,7 +431,7 @@ __global__ __launch_bounds__((CrossFewCfg<T, D>::NW * 64)) void cross_few_kernel
         st8<float>(a.part_a + (((int64_t)split * a.batch * a.kv_heads + hk) * rows + row) * D + d, w8[z]);
       } else if (d < a.dim) {
         st8_out<T>((T*)a.out + b * a.out_s[0] + head * a.out_s[1] + sq_i * a.out_s[2] + d,
-                   a.lo ? (T*)a.lo + stat * a.dim + d : nullptr, w8[z]);
+                   a.lo ? a.lo + stat * a.dim + d : nullptr, w8[z]);
       }
     }
     if (h == 0 && mt == 0) {
@@ -503,7 +503,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a, int lanes)
   const int64_t stat = ((int64_t)b * a.heads + head) * a.sq + i % a.sq;
   if (d < a.dim)
     st8_out<T>((T*)a.out + b * a.out_s[0] + head * a.out_s[1] + (i % a.sq) * a.out_s[2] + d,
-               a.lo ? (T*)a.lo + stat * a.dim + d : nullptr, acc);
+               a.lo ? a.lo + stat * a.dim + d : nullptr, acc);
   if (d == 0 && a.lse) a.lse[stat] = top == -INFINITY ? top : top + log2f(sum);
 }
 

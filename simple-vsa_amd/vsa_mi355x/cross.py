@@ -100,7 +100,7 @@ def _forward(q, k, v, lens, mask, scale, keep):
         if keep:
             lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
             if q.dtype != torch.float32:
-                lo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+                lo = torch.empty(q.shape, dtype=torch.uint8, device=dev)
         scratch = _scratch(q, k, lens, mask, 0)
         _lib.call("vsa_cross_fwd", _pack(q, k, v, lens, mask, scale), out.data_ptr(), _three(out),
                   _ptr(lo), _ptr(lse), _ptr(scratch),

@@ -272,13 +272,14 @@ def cross_fwd(q: Tensor, k: Tensor, v: Tensor, lens: Optional[Tensor], mask: Opt
     """(out, lo, lse); the last two are empty placeholders without ``save`` (lo also
     in fp32)."""
     out, lo, lse = X._forward(q, k, v, lens, mask, scale, save)
-    return (out, lo if lo is not None else _empty(q),
+    return (out, lo if lo is not None else _empty(q, torch.uint8),
             lse if lse is not None else _empty(q, torch.float32))
 
 
 @cross_fwd.register_fake
 def _(q, k, v, lens, mask, scale, save):
-    lo = q.new_empty(q.shape) if save and q.dtype != torch.float32 else _empty(q)
+    lo = (q.new_empty(q.shape, dtype=torch.uint8) if save and q.dtype != torch.float32 else
+          _empty(q, torch.uint8))
     lse = (q.new_empty(q.shape[:3], dtype=torch.float32) if save else _empty(q, torch.float32))
     return R.empty_in_order(q), lo, lse
 

@@ -444,3 +444,20 @@ def test_few_keys_take_no_more_rounding_than_their_results(n, d):
         if name != "dv":
             own = (y.to(torch.bfloat16).double() - y).norm()
             assert (x.double() - y).norm() <= 1.15 * own, name
+
+
+@pytest.mark.parametrize("dtype,n,d", [("bf16", 2000, 128), ("fp16", 1500, 64), ("bf16", 900, 256),
+                                       ("fp16", 1000, 40)])
+def test_spread_weights_lose_no_more_than_the_results_rounding(dtype, n, d):
+    """Where the weights spread over many keys, dS is far smaller than dP and delta:
+    dq stays within its own rounding, with delta from the output and its rest."""
+    from vsa_mi355x import mi355x_cross_attention
+    host = _inputs(dtype, 1, 2, 2, 300, n, d, seed=47)
+    host[3] *= 8   # (clear of fp16's subnormals: dS is about 1e-2)
+    leaves = [x.to(DEV).requires_grad_() for x in host[:3]]
+    dq, = torch.autograd.grad(mi355x_cross_attention(*leaves), leaves[:1], host[3].to(DEV))
+    ref, _ = reference(*(x.to(DEV) for x in host))
+    # a rest is off by 1/508 of the output's unit in the last place: delta by less than
+    # 2^-15 of sum |dO O|, dS by as much of P delta, against 2^-9 of dq in its rounding
+    own = (ref[1].to(DTYPES[dtype]).double() - ref[1]).norm()
+    assert (dq.double() - ref[1]).norm() <= 1.15 * own

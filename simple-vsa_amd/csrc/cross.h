@@ -13,6 +13,8 @@
 // row) takes part in a product.
 #pragma once
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "vsa_device.h"
@@ -473,6 +475,30 @@ __device__ __forceinline__ float dot_rest(typename Mma<T>::V8 g, typename Mma<T>
     sum = fmaf((float)g[e], fmaf(units, __uint_as_float(R::power(x)), x), sum);
   }
   return sum;
+}
+
+// Splits of a walk over the keys.  With `fit` workgroups that do not slow each other
+// (one a CU, of four waves), s splits take ceil(tiles s / fit) rounds of their
+// chunks, and their parts are written, read again and joined: 4.5 us and 0.4 us a
+// MB.  A chunk takes `us`; MB is one split's part.  Forward and join of 16-bit 128
+// channels, us, for the splits that fill the chip's LDS / by this rule: 12 heads,
+// 2000 queries on 512 keys 39.6 (4) / 20.7 (1), 5000 queries 54.8 (2) / 29.6 (1);
+// 8 heads, 256 queries on 10000 keys 44.4 (60) / 32.3 (16).
+inline int64_t split_keys(int64_t tiles, int64_t fit, int64_t chunks, double us, double mb) {
+  int64_t best = 1;
+  double least = 1e300;
+  auto look = [&](int64_t s) {
+    s = std::max<int64_t>(1, std::min(s, chunks));
+    const int64_t per = (chunks + s - 1) / s;
+    s = (chunks + per - 1) / per;
+    const double rounds = (double)((tiles * s + fit - 1) / fit);
+    const double cost = rounds * ((double)per * us + 1.5) + (s > 1 ? 4.5 + 0.4 * mb * (double)s : 0);
+    if (cost < least) least = cost, best = s;
+  };
+  for (int64_t s = 1; s <= 8; ++s) look(s);
+  for (int64_t k = 1; k <= 3; ++k) look(k * fit / tiles);       // k whole rounds
+  look((int64_t)std::sqrt((double)chunks * us / (0.4 * mb)));   // where both sides are equal
+  return best;
 }
 
 }  // namespace vsa

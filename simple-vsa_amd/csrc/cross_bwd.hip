@@ -604,29 +604,45 @@ void cross_dkv_kernel(CrossArgs a) {
   }
 }
 
-// out = sum of the splits' parts, in their order; one thread per eight channels
-// of a row.  blockIdx.y picks one of two results.
+// out = sum of the splits' parts, in a fixed order; blockIdx.y picks one of two
+// results.  A row has D / 8 threads of eight channels, times `lanes` that sum every
+// lanes-th split each and meet in LDS (256 splits of 128 rows by one thread a
+// piece: 66 us, longer than the pass).
 struct SumArgs {
   const float* part[2];
   void* out[2];
   int64_t s[2][3];
   int64_t rows;        // batch * heads * tokens
-  int splits, heads, tokens, dim;
+  int splits, heads, tokens, dim, lanes;
 };
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cross_sum_kernel(SumArgs a) {
+  constexpr int W = D / 8;
+  __shared__ float acc_s[256][9];
   const int y = blockIdx.y;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = id / (D / 8);
-  const int d = (int)(id % (D / 8)) * 8;
-  if (row >= a.rows || d >= a.dim) return;
+  const int d = threadIdx.x % W * 8, lane = threadIdx.x / W % a.lanes;
+  const int64_t row = (int64_t)blockIdx.x * (256 / W / a.lanes) + threadIdx.x / W / a.lanes;
+  const bool on = row < a.rows && d < a.dim;
   float acc[8] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float* p = a.part[y] + (s * a.rows + row) * D + d;
-    const f32x4 u = *reinterpret_cast<const f32x4*>(p), v = *reinterpret_cast<const f32x4*>(p + 4);
+  if (on) {
+#pragma unroll 4   // (loads ahead of the sums)
+    for (int s = lane; s < a.splits; s += a.lanes) {
+      const float* p = a.part[y] + (s * a.rows + row) * D + d;
+      const f32x4 u = *reinterpret_cast<const f32x4*>(p), v = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += u[e], acc[4 + e] += v[e];
+      for (int e = 0; e < 4; ++e) acc[e] += u[e], acc[4 + e] += v[e];
+    }
   }
+  if (a.lanes > 1) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc_s[threadIdx.x][e] = acc[e];
+    __syncthreads();
+    if (lane) return;
+    for (int x = 1; x < a.lanes; ++x)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += acc_s[threadIdx.x + x * W][e];
+  }
+  if (!on) return;
   const int64_t bh = row / a.tokens, t = row % a.tokens;
   st8<T>((T*)a.out[y] + bh / a.heads * a.s[y][0] + bh % a.heads * a.s[y][1] + t * a.s[y][2] + d, acc);
 }
@@ -639,13 +655,6 @@ struct Plan {
   int k_nw, k_splits, k_per_head;      // dK / dV
   int64_t q_tiles, k_tiles;
 };
-
-int64_t splits_for(int64_t tiles, int64_t fit, int64_t steps, int64_t least) {
-  int64_t s = tiles >= fit ? 1 : fit / tiles;
-  s = std::max<int64_t>(1, std::min(s, steps / least));
-  const int64_t per = (steps + s - 1) / s;
-  return (steps + per - 1) / per;
-}
 
 // Splits of the pass over the queries.  With `fit` workgroups at once, s splits
 // take ceil(tiles s / fit) rounds of steps / s items and a workgroup's own cost
@@ -682,9 +691,9 @@ Plan bwd_plan(const vsa_cross* c) {
   p.q_nw = rows <= 32 && !wide ? 1 : rows <= 64 ? 2 : 4;
   p.q_per_head = (int)((rows + 32 * p.q_nw - 1) / (32 * p.q_nw));
   p.q_tiles = (int64_t)c->batch * c->kv_heads * p.q_per_head;
-  const int lds = 4 * 32 * p.kd * es;
-  const int64_t fit = (int64_t)cu_count() * std::max(1, std::min(160 * 1024 / lds, 8 / p.q_nw));
-  p.q_splits = (int)splits_for(p.q_tiles, fit, (c->skv + 31) / 32, 4);
+  const double us = es == 4 ? 0.048 * c->head_dim : 0.35 + 0.0055 * p.kd;
+  p.q_splits = (int)split_keys(p.q_tiles, (int64_t)cu_count() * (4 / p.q_nw), (c->skv + 31) / 32, us,
+                               (double)c->batch * c->kv_heads * rows * p.kd * 4e-6);
   const int wave_keys = es == 2 && p.kd == 64 ? 64 : 32;
   p.k_nw = wide ? 2 : p.kd == 256 ? 4 : c->skv <= wave_keys ? 1 : c->skv <= 2 * wave_keys ? 2 : 4;
   p.k_per_head = (int)((c->skv + wave_keys * p.k_nw - 1) / (wave_keys * p.k_nw));
@@ -713,8 +722,10 @@ int64_t cross_bwd_parts(const vsa_cross* c) {
 }
 
 template <typename T, int D>
-static int launch_sum(const SumArgs& a, int results, hipStream_t s) {
-  const int64_t grid = (a.rows * (D / 8) + 255) / 256;
+static int launch_sum(SumArgs a, int results, hipStream_t s) {
+  a.lanes = 1;   // a power of two, four splits or more each
+  while (8 * a.lanes <= a.splits && a.lanes < 256 / (D / 8)) a.lanes *= 2;
+  const int64_t per = 256 / (D / 8) / a.lanes, grid = (a.rows + per - 1) / per;
   if (grid > (1LL << 31) - 1) return VSA_ERR_SHAPE;
   hipLaunchKernelGGL((cross_sum_kernel<T, D>), dim3((unsigned)grid, results), dim3(256), 0, s, a);
   return vsa_check_launch();

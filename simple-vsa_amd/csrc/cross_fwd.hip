@@ -555,15 +555,11 @@ Plan fwd_plan(const vsa_cross* c) {
   p.nw = rows <= 32 && !wide ? 1 : rows <= 64 ? 2 : 4;
   p.per_head = (int)((rows + 32 * p.nw - 1) / (32 * p.nw));
   p.tiles = heads * p.per_head;
-  // workgroups that the chip holds at once, by their LDS
+  // (measured with 4 waves on an idle chip; fp32 leaves out channels past the head dim)
   const int kc = fwd_kc(c, p.kd, p.nw);
-  const int lds = 4 * kc * p.kd * (c->dtype == VSA_F32 ? 4 : 2);
-  const int64_t fit = (int64_t)cu_count() * std::max(1, std::min(160 * 1024 / lds, 16 / p.nw));
-  const int64_t chunks = (c->skv + kc - 1) / kc;
-  int64_t splits = p.tiles >= fit ? 1 : fit / p.tiles;
-  splits = std::max<int64_t>(1, std::min(splits, chunks / 4));
-  const int64_t per = (chunks + splits - 1) / splits;
-  p.splits = (int)((chunks + per - 1) / per);
+  const double us = c->dtype == VSA_F32 ? 0.036 * c->head_dim : (0.1 + 0.0052 * p.kd) * kc / 32;
+  p.splits = (int)split_keys(p.tiles, (int64_t)cu_count() * (4 / p.nw), (c->skv + kc - 1) / kc, us,
+                             (double)heads * rows * p.kd * 4e-6);
   return p;
 }
 

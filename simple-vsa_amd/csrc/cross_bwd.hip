@@ -358,26 +358,42 @@ void cross_dkv_kernel(CrossArgs a) {
 
   // An item's copy: descriptors of its rows, and this lane's statistic (lanes of
   // half 0 the lse, of half 1 the delta; every wave copies them, so that all
-  // wait for the same number of loads).
+  // wait for the same number of loads).  Addresses go from item to item by
+  // additions: a wave issues an instruction at a time, and products of 64 bits
+  // for every item took a fifth of its step.
   struct Item {
     typename C::Copy::Src q, g;
     const float* stat;
   };
-  int head_i = first / qt, row_i = first % qt;   // of the next item to copy
+  const int head_f = first / qt, row_f = first % qt;
+  const int head0 = kh * a.group + head_f;
+  const T* qhead = (const T*)a.q.p + b * a.q.b + head0 * a.q.h;
+  const T* ghead = (const T*)a.dout.p + b * a.dout.b + head0 * a.dout.h;
+  const float* shead = (h ? a.delta : a.lse) + ((int64_t)b * a.heads + head0) * a.sq + r;
+  // of the next item to copy
+  const T* qrows = qhead + (int64_t)row_f * 32 * a.q.s;
+  const T* grows = ghead + (int64_t)row_f * 32 * a.dout.s;
+  const float* stat = shead + row_f * 32;
+  int left = a.sq - row_f * 32;
+  const int64_t qstep = 32 * a.q.s, gstep = 32 * a.dout.s;
   auto next_item = [&]() __attribute__((always_inline)) {
-    const int head = kh * a.group + head_i, s0 = row_i * 32, left = a.sq - s0;
     Item it;
-    it.q = qcopy.rows((const T*)a.q.p + b * a.q.b + head * a.q.h + (int64_t)s0 * a.q.s, left);
-    it.g = gcopy.rows((const T*)a.dout.p + b * a.dout.b + head * a.dout.h + (int64_t)s0 * a.dout.s,
-                      left);
-    it.stat = (h ? a.delta : a.lse) + ((int64_t)b * a.heads + head) * a.sq + s0 + r;
-    if (r >= left) it.stat = kPastStats + h;
+    it.q = qcopy.rows(qrows, left);
+    it.g = gcopy.rows(grows, left);
+    it.stat = r < left ? stat : kPastStats + h;
     return it;
   };
   // (past the last item its copy is made again, into a stage that no one reads)
   auto advance = [&](int i) __attribute__((always_inline)) {
     if (i >= items) return;
-    if (++row_i == qt) row_i = 0, ++head_i;
+    left -= 32, qrows += qstep, grows += gstep, stat += 32;
+    if (left <= 0) {
+      keep_branch();
+      left = a.sq;
+      qrows = qhead += a.q.h;
+      grows = ghead += a.dout.h;
+      stat = shead += a.sq;
+    }
   };
   auto piece = [&](const Item& it, int stage, int p) __attribute__((always_inline)) {
     const uint32_t to = lds0 + stage * C::STAGE;

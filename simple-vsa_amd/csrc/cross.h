@@ -56,15 +56,30 @@ __device__ __forceinline__ typename Mma<T>::V8 pack_op(const float* v) {
   }
 }
 
-// Eight values as an operand, and what rounding them to T left over as another.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::V8 zero8() {
+  typename Mma<T>::V8 z = {};
+  return z;
+}
+
+// Eight values as an operand, and what rounding them to T left over as another.  (The
+// pairs are opaque: unpacked by the compiler each value is rounded a second time.)
 template <typename T>
 __device__ __forceinline__ void pack_both(const float* v, typename Mma<T>::V8& hi,
                                           typename Mma<T>::V8& lo) {
-  hi = pack_op<T>(v);
-  float rest[8];
+  if constexpr (sizeof(T) == 4) {
+    hi = pack_op<T>(v);
+    lo = zero8<T>();
+  } else {
+    u32x4 w = __builtin_bit_cast(u32x4, pack_op<T>(v));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) rest[e] = v[e] - (float)hi[e];
-  lo = pack_op<T>(rest);
+    for (int i = 0; i < 4; ++i) w[i] = opaque(w[i]);
+    hi = as_vec8<T>(w);
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) rest[e] = fmaf((float)hi[e], -1.f, v[e]);
+    lo = pack_op<T>(rest);
+  }
 }
 
 // 8 consecutive elements at a 16-byte aligned address
@@ -76,11 +91,6 @@ __device__ __forceinline__ typename Mma<T>::V8 ld8(const T* p) {
   } else {
     return as_vec8<T>(*reinterpret_cast<const u32x4*>(p));
   }
-}
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::V8 zero8() {
-  typename Mma<T>::V8 z = {};
-  return z;
 }
 
 // Wide rows leave no registers to read many operands ahead: without a fence after

@@ -5,7 +5,7 @@
 //   dQ = scale dS K      dK = scale dS^T Q      dV = P^T dO
 //
 // dQ's pass is bound by reading q, dO, O and its rest and writing dQ up to a few
-// hundred keys (24 heads x 16k queries of 128 channels: 0.13 ms on 32 keys, 0.26 on
+// hundred keys (24 heads x 16k queries of 128 channels: 0.12 ms on 32 keys, 0.26 on
 // 512), then by its products and exponentials (0.30 us a key); the other pass by
 // the latter (0.36 us a key).
 //
@@ -93,7 +93,7 @@ void cross_dq_kernel(CrossArgs a) {
     const T* grow = (const T*)a.dout.p + b * a.dout.b + head * a.dout.h + sq_i * a.dout.s;
     const T* orow = (const T*)a.o.p + b * a.o.b + head * a.o.h + sq_i * a.o.s;
     // tensor by tensor: the loads of a row's 128-byte lines follow each other (16k
-    // queries on 32 keys, head dim 128: 0.160 -> 0.133 ms)
+    // queries on 32 keys, head dim 128: 0.160 -> 0.133 ms; 0.122 with the rests as bytes)
     auto load = [&](V8 (&f)[D / 16], const T* p) __attribute__((always_inline)) {
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
@@ -257,8 +257,8 @@ void cross_dq_kernel(CrossArgs a) {
 // step i multiplies S and dP of item i + 1 while it works out P and dS of item
 // i, then dV and dK of item i; operands are read from LDS AHEAD products before
 // their use, and the copy of item i + 3 is spread over the second half.
-// 2 x 12 heads, 16k queries on 512 and 256 keys, head dim 128: 0.25 ms, without
-// the overlap 0.45; on 2048 keys 1.1 PFLOP/s.
+// 2 x 12 heads, 16k queries on 512 and 256 keys, head dim 128: 0.23 ms (0.45 without
+// the overlap); on 2048 keys 1.1 PFLOP/s.
 template <typename T, int D, int NW>
 struct CrossDkvCfg {
   static constexpr int NT = NW * 64;
@@ -277,9 +277,9 @@ struct CrossDkvCfg {
   static constexpr int NC = 4 * (DA / 32);               // dO and Q columns
   static constexpr int NV = 16 * KT;                     // P values of a lane per item
   // Up to 64 keys (128 at head dim 64) the pass reads Q and dO for longer than it
-  // multiplies, and dK takes what rounding dS leaves over as well: 16k queries on 32
-  // keys 42 -> 45 us at head dim 128, 29 -> 33 on 64 at head dim 64, dK off 1.7e-3 of
-  // its norm instead of 2.4e-3.  For more keys it stays out (512: 241 -> 288 us).
+  // multiplies, and dK takes what rounding dS leaves over as well: 24 heads x 16k
+  // queries on 32 keys 42 us, 3 of them for it, on 64 keys at head dim 64 32 us, 4 of
+  // them; dK is off 1.7e-3 of its norm instead of 2.4e-3.  For more keys it stays out (512: 241 -> 288 us).
   static constexpr bool BOTH = PIPE && NW <= 2;
   static constexpr int AHEAD = D > 128 || (KT > 1 && BOTH) ? 4 : KT > 1 ? 6 : 12;
 };

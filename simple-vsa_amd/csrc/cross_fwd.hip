@@ -18,9 +18,9 @@
 //
 // Bound by the products and exponentials a tile takes, with the reading of q and
 // the writing of O at its start and end on top where it has few chunks: 40 heads x
-// 41k queries of 128 channels on 512 keys 0.50 ms, 860 TFLOP/s (matrix core 49 %
-// of the time, vector unit 44 %, q and O alone 0.17 ms); on 2048 keys of 24 heads x
-// 16k queries 0.42 ms, 980.
+// 41k queries of 128 channels on 512 keys 0.50 ms, 860 TFLOP/s (matrix core busy
+// for 45 % of the cycles, at the 1.7 GHz that the chip's power allows; q and O alone
+// 0.17 ms); on 2048 keys of 24 heads x 16k queries 0.42 ms, 980.
 #include <algorithm>
 #include <type_traits>
 
@@ -33,6 +33,9 @@ constexpr float kSlack = 8.0f;  // log2 units
 template <typename T, int D, int NW>
 struct CrossFwdCfg {
   static constexpr int NT = NW * 64;
+  // 128 channels: 32 keys leave registers for three waves a SIMD, 64 for two (40 heads
+  // x 41k queries on 512 keys 0.508 / 0.540 ms).  64 channels: 64 keys 582 us, 32 598
+  // (24 heads x 41k queries on 2048), 13.1 / 15.2 (12 heads x 2000 on 512).
   static constexpr int KC = sizeof(T) == 2 && D < 128 && NW == 4 ? 64 : 32;
   static constexpr int NSM = KC / 32;
   static constexpr int TILE = KC * D * (int)sizeof(T);   // bytes of a K (or V) chunk

@@ -145,3 +145,25 @@ def test_lengths_of_64_bits_are_clamped_before_they_lose_bits():
     assert _lens(lens, 7, lens.device).tolist() == [7, 0, 7, 5, 0]
     assert _lens(lens, 7, lens.device).dtype == torch.int32
     assert _lens(None, 7, lens.device) is None
+
+
+def test_the_outputs_rest_and_gradients_are_aligned():
+    """The rest of the output is read eight bytes at a time; rows on 16 bytes."""
+    lib = _lib.load()
+    buf = torch.zeros(256)
+    p = (buf.data_ptr() + 255) // 256 * 256
+    st = (ctypes.c_int64 * 3)(64, 64, 64)
+    s3 = ctypes.addressof(st)
+    c = Cross()
+    c.q = c.k = c.v = p
+    c.q_stride[:] = c.k_stride[:] = c.v_stride[:] = [64, 64, 64]
+    c.sq, c.skv, c.batch, c.heads, c.kv_heads, c.head_dim, c.scale = 4, 6, 2, 4, 2, 64, 0.125
+    at = ctypes.addressof(c)
+    assert lib.vsa_cross_fwd(at, p, s3, p + 4, None, p, None) == -7
+    assert lib.vsa_cross_fwd(at, p, s3, None, p + 2, p, None) == -7
+    assert lib.vsa_cross_fwd(at, p, s3, None, None, p + 128, None) == -7
+    good = [at, p, s3, p, p, s3, p, p, s3, p, s3, p, s3, p, None]
+    for i, off in ((1, 8), (3, 4), (4, 8), (6, 2), (7, 8), (9, 8), (11, 8), (13, 128)):
+        bad = list(good)
+        bad[i] = p + off
+        assert lib.vsa_cross_bwd(*bad) == -7, i

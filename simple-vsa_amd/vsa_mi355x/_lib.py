@@ -94,6 +94,7 @@ class VsaOp(ctypes.Structure):
 ROTARY_AXES = struct.Struct("4i4d" * 3)
 ROTARY_OP = struct.Struct("7P16q8i")
 CROSS = struct.Struct("5P12q5if")
+CROSS_POINTERS = struct.Struct("5P")   # its first part
 STRIDES = struct.Struct("3q")
 
 

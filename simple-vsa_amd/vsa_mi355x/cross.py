@@ -14,7 +14,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
@@ -23,40 +23,88 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .launch import _ptr, _workspace, on_device
 from .mi355x import KERNEL_DTYPES, _i32
-from .rotary import empty_in_order, strides
+from .rotary import empty_in_order, token_order
 
 MAX_HEAD_DIM = 256
 MAX_TOKENS = (1 << 31) - 256
 MAX_SCALE = 2.0 ** 127   # times log2(e) it stays finite in fp32
 
 
+def _far(stride: int, element_size: int) -> bool:
+    """Whether a tile's rows lie out of reach of a 32-bit offset."""
+    return stride > (1 << 30) // (64 * element_size)
+
+
 def _rows16(x: Tensor) -> Tensor:
     """x itself where the kernels read its rows in place (channels next to each
-    other, every row 16-byte aligned, a tile's rows within reach of a 32-bit
-    offset), else a dense copy."""
+    other, every row 16-byte aligned, a tile's rows within reach), else a dense
+    copy in x's order of heads and tokens."""
     if x.is_contiguous():
         return x if x.data_ptr() % 16 == 0 else x.clone()
     es = x.element_size()
     if x.stride(3) == 1 and x.data_ptr() % 16 == 0:
-        b, h, s = _strides(x)
-        if (b | h | s) * es % 16 == 0 and x.shape[3] <= s <= (1 << 30) // (64 * es):
+        b, h, s = _strides(x.shape, x.stride())
+        if (b | h | s) * es % 16 == 0 and x.shape[3] <= s and not _far(s, es):
             return x
+    if token_order(x) and not _far(x.shape[1] * x.shape[3], es):
+        return x.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
     return x.clone(memory_format=torch.contiguous_format)
 
 
-def _strides(x: Tensor):
-    """Strides for the C ABI; those of a row where there is one token."""
-    b, h, s = strides(x)
-    return b, h, s if x.shape[2] > 1 else x.shape[3]
+def _strides(shape, stride):
+    """Strides of batch, head and token for the C ABI: 0 for a dimension of one, those
+    of a row where there is one token."""
+    (b, h, s, d), (sb, sh, ss, _) = shape, stride
+    return sb if b > 1 else 0, sh if h > 1 else 0, ss if s > 1 else d
 
 
-def _pack(q, k, v, lens, mask, scale) -> bytes:
-    b, h, sq, d = q.shape
-    return _lib.CROSS.pack(
+def _three(x: Tensor) -> bytes:
+    return _lib.STRIDES.pack(*_strides(x.shape, x.stride()))
+
+
+def _dense(shape, stride) -> bytes:
+    """The strides of ``empty_in_order``'s result."""
+    b, h, s, d = shape
+    if h > 1 and s > 1 and stride[1] < stride[2]:
+        return _lib.STRIDES.pack(*_strides(shape, (s * h * d, d, h * d, 1)))
+    return _lib.STRIDES.pack(*_strides(shape, (h * s * d, s * d, d, 1)))
+
+
+class _Plan(NamedTuple):
+    """What a call takes from its sizes alone: the struct behind its pointers, the
+    strides of the results, bytes of scratch."""
+    rest: bytes
+    q: bytes
+    k: bytes
+    v: bytes
+    forward: int
+    backward: int
+
+
+@functools.lru_cache(maxsize=256)
+def _plan_of(q, qs, k, ks, vs, lens, mask, dtype, scale, device) -> _Plan:
+    """``device`` is the current one: the splits follow its number of CUs."""
+    (b, h, sq, d), (_, hk, skv, _) = q, k
+    rest = _lib.CROSS.pack(0, 0, 0, 0, 0, *_strides(q, qs), *_strides(k, ks), *_strides(k, vs), mask or 0, sq,
+                           skv, b, h, hk, d, dtype, scale)[_lib.CROSS_POINTERS.size:]
+    n = (ctypes.c_int64 * 2)()
+    at = ctypes.addressof(n)
+    # a pointer's presence is all that is read
+    _lib.call("vsa_cross_sizes", _lib.CROSS_POINTERS.pack(256, 256, 256, 256 * lens, 256 * (mask is not None))
+              + rest, at, at + 8)
+    return _Plan(rest, _dense(q, qs), _dense(k, ks), _dense(k, vs), *n)
+
+
+def _plan(q, k, v, lens, mask, scale) -> _Plan:
+    return _plan_of(q.shape, q.stride(), k.shape, k.stride(), v.stride(), lens is not None,
+                    None if mask is None else mask.stride(0), _lib.DTYPE_CODES[q.dtype], scale,
+                    q.device.index)
+
+
+def _pointers(q, k, v, lens, mask) -> bytes:
+    return _lib.CROSS_POINTERS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if lens is None else lens.data_ptr(),
-        0 if mask is None else mask.data_ptr(), *_strides(q), *_strides(k), *_strides(v),
-        0 if mask is None else mask.stride(0), sq, k.shape[2], b, h, k.shape[1], d,
-        _lib.DTYPE_CODES[q.dtype], scale)
+        0 if mask is None else mask.data_ptr())
 
 
 def _lens(kv_lens: Optional[Tensor], skv: int, device) -> Optional[Tensor]:
@@ -66,44 +114,21 @@ def _lens(kv_lens: Optional[Tensor], skv: int, device) -> Optional[Tensor]:
     return _i32(kv_lens.clamp(0, skv) if kv_lens.dtype is torch.int64 else kv_lens, device)
 
 
-def _three(x: Tensor) -> bytes:
-    return _lib.STRIDES.pack(*_strides(x))
-
-
-@functools.lru_cache(maxsize=256)
-def _sizes(b, h, hk, sq, skv, d, lens, masked, dtype, device):
-    """Bytes of (forward scratch, backward scratch) on ``device``, the current one
-    (the splits follow its number of CUs)."""
-    # a pointer's presence is all that is read
-    c = _lib.CROSS.pack(256, 256, 256, 256 if lens else 0, 256 if masked else 0, *(0, 0, 256) * 3, 0, sq, skv, b, h,
-                        hk, d, dtype, 1.0)
-    n = (ctypes.c_int64 * 2)()
-    at = ctypes.addressof(n)
-    _lib.call("vsa_cross_sizes", c, at, at + 8)
-    return tuple(n)
-
-
-def _scratch(q, k, lens, mask, which: int) -> Optional[Tensor]:
-    b, h, sq, d = q.shape
-    return _workspace(_sizes(b, h, k.shape[1], sq, k.shape[2], d, lens is not None,
-                             mask is not None, _lib.DTYPE_CODES[q.dtype], q.device.index)[which],
-                      q.device)
-
-
 def _forward(q, k, v, lens, mask, scale, keep):
     """(out, lo, lse); the last two only where the backward needs them (``keep``)."""
     dev = q.device
     with on_device(dev):
-        out = empty_in_order(q)
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        out = empty_in_order(q)
         lo = lse = None
         if keep:
             lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
             if q.dtype != torch.float32:
                 lo = torch.empty(q.shape, dtype=torch.uint8, device=dev)
-        scratch = _scratch(q, k, lens, mask, 0)
-        _lib.call("vsa_cross_fwd", _pack(q, k, v, lens, mask, scale), out.data_ptr(), _three(out),
-                  _ptr(lo), _ptr(lse), _ptr(scratch),
+        plan = _plan(q, k, v, lens, mask, scale)
+        scratch = _workspace(plan.forward, dev)
+        _lib.call("vsa_cross_fwd", _pointers(q, k, v, lens, mask) + plan.rest, out.data_ptr(),
+                  plan.q, _ptr(lo), _ptr(lse), _ptr(scratch),
                   torch._C._cuda_getCurrentRawStream(dev.index))
     return out, lo, lse
 
@@ -111,15 +136,16 @@ def _forward(q, k, v, lens, mask, scale, keep):
 def _backward(q, k, v, lens, mask, scale, out, lo, lse, dout):
     dev = q.device
     with on_device(dev):
-        dq, dk, dv = (empty_in_order(x) for x in (q, k, v))
         # (the saved ones too: a saved-tensor hook may give back other addresses)
         q, k, v, out, dout = (_rows16(x) for x in (q, k, v, out, dout))
+        dq, dk, dv = (empty_in_order(x) for x in (q, k, v))
         lo = lo if lo is None else _rows16(lo.contiguous())
-        scratch = _scratch(q, k, lens, mask, 1)
-        _lib.call("vsa_cross_bwd", _pack(q, k, v, lens, mask, scale), out.data_ptr(), _three(out),
-                  _ptr(lo), dout.data_ptr(), _three(dout), lse.data_ptr(), dq.data_ptr(),
-                  _three(dq), dk.data_ptr(), _three(dk), dv.data_ptr(), _three(dv), _ptr(scratch),
-                  torch._C._cuda_getCurrentRawStream(dev.index))
+        plan = _plan(q, k, v, lens, mask, scale)
+        scratch = _workspace(plan.backward, dev)
+        _lib.call("vsa_cross_bwd", _pointers(q, k, v, lens, mask) + plan.rest, out.data_ptr(),
+                  _three(out), _ptr(lo), dout.data_ptr(), _three(dout), lse.data_ptr(),
+                  dq.data_ptr(), plan.q, dk.data_ptr(), plan.k, dv.data_ptr(), plan.v,
+                  _ptr(scratch), torch._C._cuda_getCurrentRawStream(dev.index))
     return dq, dk, dv
 
 

@@ -461,3 +461,30 @@ def test_spread_weights_lose_no_more_than_the_results_rounding(dtype, n, d):
     # 2^-15 of sum |dO O|, dS by as much of P delta, against 2^-9 of dq in its rounding
     own = (ref[1].to(DTYPES[dtype]).double() - ref[1]).norm()
     assert (dq.double() - ref[1]).norm() <= 1.15 * own
+
+
+@pytest.mark.parametrize("d", [64, 60])
+def test_copied_views_keep_their_order_with_and_without_gradients(d):
+    """Token-major views whose rows do not start on 16 bytes are copied; the result
+    and the gradients are dense in the order of the view all the same."""
+    from vsa_mi355x import mi355x_cross_attention
+    b, h, sq, n = 2, 3, 33, 20
+    host = _inputs("bf16", b, h, h, sq, n, d, seed=53)
+
+    def odd(x):   # token-major, 2 bytes off
+        buf = torch.zeros(x.numel() + 1, dtype=x.dtype, device=DEV)
+        view = buf[1:].view(x.shape[0], x.shape[2], x.shape[1], d).transpose(1, 2)
+        view.copy_(x)
+        return view
+    q, k, v, do = (odd(x) for x in host)
+    want = torch.empty(b, sq, h, d).transpose(1, 2).stride()
+    with torch.no_grad():
+        plain = mi355x_cross_attention(q, k, v)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = mi355x_cross_attention(*leaves)
+    if d % 8 == 0:
+        assert plain.stride() == out.stride() == want
+    assert torch.equal(plain, out) and plain.stride() == out.stride()
+    grads = torch.autograd.grad(out, leaves, do)
+    ref, tol = reference(*(x.to(DEV) for x in host))
+    _check(NAMES, [out, *grads], ref, tol)

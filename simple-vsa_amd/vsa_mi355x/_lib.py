@@ -93,6 +93,7 @@ class VsaOp(ctypes.Structure):
 # vsa_rotary_op and vsa_cross of the header, fields in order.
 ROTARY_AXES = struct.Struct("4i4d" * 3)
 ROTARY_OP = struct.Struct("7P16q8i")
+ROTARY_POINTERS = struct.Struct("7P")   # its first part
 CROSS = struct.Struct("5P12q5if")
 CROSS_POINTERS = struct.Struct("5P")   # its first part
 STRIDES = struct.Struct("3q")

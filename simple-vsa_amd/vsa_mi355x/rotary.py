@@ -123,10 +123,21 @@ def empty_in_order(x: Tensor) -> Tensor:
     return torch.empty((b, h, s, d), dtype=x.dtype, device=x.device)
 
 
-def strides(x: Tensor) -> Tuple[int, int, int]:
+def _strides(shape, stride) -> Tuple[int, int, int]:
     """Strides of batch, head and token for the C ABI; 0 for a dimension of one."""
-    (b, h, s, _), (sb, sh, ss, _) = x.shape, x.stride()
+    (b, h, s, _), (sb, sh, ss, _) = shape, stride
     return (sb if b > 1 else 0, sh if h > 1 else 0, ss if s > 1 else 0)
+
+
+@functools.lru_cache(maxsize=256)
+def _rest_of(q, qs, qo, k, ks, ko, table, positions, wide, interleaved, inverse, dtype) -> bytes:
+    """The struct behind its pointers, from shapes and strides alone."""
+    b, h, s, d = q
+    rows, pairs = table
+    return _lib.ROTARY_OP.pack(
+        0, 0, 0, 0, 0, 0, 0, *_strides(q, qs), *_strides(k or q, ks), *_strides(q, qo),
+        *_strides(k or q, ko), s if positions == 2 else 0, b, s, rows, h, k[1] if k else 0, d,
+        2 * pairs, interleaved, inverse, wide, dtype)[_lib.ROTARY_POINTERS.size:]
 
 
 def _rotate(q, k, cos, sin, positions, interleaved, inverse):
@@ -135,22 +146,20 @@ def _rotate(q, k, cos, sin, positions, interleaved, inverse):
     if q.stride(3) != 1:
         q = q.contiguous()
     k_out = None
-    kk, ko, hk = q, q_out, 0
+    kk, ko = q, q_out
     if k is not None:
         k_out = ko = empty_in_order(k)
-        kk, hk = k if k.stride(3) == 1 else k.contiguous(), k.shape[1]
-    b, h, s, d = q.shape
-    rows, pairs = cos.shape
-    op = _lib.ROTARY_OP.pack(
+        kk = k if k.stride(3) == 1 else k.contiguous()
+    rest = _rest_of(q.shape, q.stride(), q_out.stride(), None if k is None else kk.shape, kk.stride(),
+                    ko.stride(), cos.shape, 0 if positions is None else positions.dim(),
+                    positions is not None and positions.dtype is torch.int64, interleaved, inverse,
+                    _lib.DTYPE_CODES[q.dtype])
+    pointers = _lib.ROTARY_POINTERS.pack(
         q.data_ptr(), kk.data_ptr(), q_out.data_ptr(), ko.data_ptr(), cos.data_ptr(),
-        sin.data_ptr(), 0 if positions is None else positions.data_ptr(), *strides(q),
-        *strides(kk), *strides(q_out), *strides(ko),
-        0 if positions is None or positions.dim() == 1 else s, b, s, rows, h, hk, d, 2 * pairs,
-        interleaved, inverse, positions is not None and positions.dtype is torch.int64,
-        _lib.DTYPE_CODES[q.dtype])
+        sin.data_ptr(), 0 if positions is None else positions.data_ptr())
     dev = q.device
     with on_device(dev):
-        _lib.call("vsa_rotary", op, torch._C._cuda_getCurrentRawStream(dev.index))
+        _lib.call("vsa_rotary", pointers + rest, torch._C._cuda_getCurrentRawStream(dev.index))
     return q_out, k_out
 
 
